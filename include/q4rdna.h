@@ -37,7 +37,8 @@ typedef enum q4rdna_status {
     Q4RDNA_OK = 0,
     Q4RDNA_ERR_INVALID_ARGUMENT = 1, /* null pointer, non-positive size, unknown op */
     Q4RDNA_ERR_SHAPE = 2,            /* N % 32 != 0, K % 64 != 0, or shape mismatch */
-    Q4RDNA_ERR_ALIGNMENT = 3,        /* tiles not 16-byte aligned, x/y/add not 8-byte aligned */
+    Q4RDNA_ERR_ALIGNMENT = 3,        /* tiles not 16-byte aligned, x/y/add not 8-byte aligned,
+                                        cache operands or strides not 16-byte multiples */
     Q4RDNA_ERR_WORKSPACE = 4,        /* workspace missing or smaller than q4rdna_workspace_bytes */
     Q4RDNA_ERR_UNSUPPORTED = 5,      /* batch B outside [1, Q4RDNA_MAX_BATCH] */
     Q4RDNA_ERR_CUDA = 6,             /* a CUDA call failed (launch, copy, allocation) */
@@ -334,6 +335,122 @@ q4rdna_status q4rdna_ipc_free(void *dev_ptr);
  * (q4rdna.format.write_sidecar). */
 q4rdna_status q4rdna_pack_bf16(const uint16_t *bf16, uint8_t *tiles, int N, int K, q4rdna_stream_t stream);
 
+/* ---- key/value cache in 8 bits: append and attention ----
+ * What a decoder layer does between its q/k/v products and its output product:
+ * per-head RMSNorm and rotation of q and k, the append of k and v to a paged
+ * cache, and the attention over that cache.  No reference counterpart (the
+ * reference leaves these to llama.cpp).
+ *
+ * Cache layout.  A tile holds 16 consecutive tokens of one kv head:
+ *   f32 key scale, f32 value scale, 8 unused bytes, key codes [16][head_dim],
+ *   value codes [16][head_dim]                        (16 + 32 * head_dim bytes)
+ * and a number is scale * code.  Codes are int8 in [-127, 127] or e4m3 in
+ * [-448, 448].  A page is [kv_heads][page_tokens / 16] tiles; the cache is
+ * `pages` pages back to back, 16-byte aligned.  Token p of sequence s lives in
+ * page page_table[s * table_stride + p / page_tokens], tile p % page_tokens / 16,
+ * row p % 16.  head_dim is 64, 128 or 256; page_tokens a power of two in
+ * [16, 256].  A tile whose numbers are all below 2^-100 of the largest code is
+ * stored as zeros with scale 0. */
+#define Q4RDNA_KV_BLOCK 16
+typedef enum q4rdna_kv_format { Q4RDNA_KV_INT8 = 0, Q4RDNA_KV_E4M3 = 1 } q4rdna_kv_format;
+/* Element type of q, k, v and the outputs of the cache operators. */
+typedef enum q4rdna_type { Q4RDNA_F32 = 0, Q4RDNA_F16 = 1, Q4RDNA_BF16 = 2 } q4rdna_type;
+/* Rotation of element pairs: (i, i + rotary_dim / 2) or (2i, 2i + 1). */
+typedef enum q4rdna_rope { Q4RDNA_ROPE_NEOX = 0, Q4RDNA_ROPE_NORM = 1 } q4rdna_rope;
+
+typedef struct q4rdna_kv_cache {
+    uint8_t *tiles;
+    int pages;
+    int page_tokens;
+    int kv_heads;
+    int head_dim;
+    int format; /* q4rdna_kv_format */
+} q4rdna_kv_cache;
+
+/* Which tokens of which sequences a call deals with.  Sequence s owns the rows
+ * q_start[s] .. q_start[s + 1] - 1 of q, k and v (q_start == NULL: row s), and
+ * lengths[s] is its number of tokens with these, the last ones, counted: row
+ * q_start[s] + i stands for token lengths[s] - n + i of the sequence's n new
+ * ones.  A negative token (a padded row of a batch: lengths[s] < n) is not
+ * stored and sees nothing.  The arrays are device memory and are read when the
+ * kernels run, so a captured call takes the values of the replay.  max_length
+ * (0: table_stride * page_tokens) bounds every length on the host's side. */
+typedef struct q4rdna_kv_batch {
+    const int32_t *page_table; /* [sequences][table_stride] */
+    const int32_t *lengths;    /* [sequences] */
+    const int32_t *q_start;    /* [sequences + 1], ascending, or NULL */
+    int sequences;
+    int table_stride;
+    int max_length;
+} q4rdna_kv_batch;
+
+/* Rows of [heads][head_dim], head after head; strides are elements from row to
+ * row.  All pointers and strides are multiples of 16 bytes. */
+typedef struct q4rdna_kv_append_args {
+    int type;   /* q4rdna_type of k, v, q and q_out */
+    int tokens; /* rows of k, v and q */
+    int heads;  /* query heads (a multiple of kv_heads), or 0 without q */
+    const void *k, *v, *q;
+    void *q_out; /* may be q itself */
+    int64_t k_stride, v_stride, q_stride, q_out_stride;
+    const float *inv_freq; /* [rotary_dim / 2], or NULL: no rotation */
+    int rotary_dim;        /* a multiple of 16, at most head_dim; 0: head_dim */
+    int rope;              /* q4rdna_rope */
+    const int32_t *positions; /* [tokens] rotation position of each row, or NULL: its token number */
+    const float *q_norm, *k_norm; /* [head_dim] RMSNorm weights, or NULL: no norm */
+    float norm_eps;
+} q4rdna_kv_append_args;
+
+typedef struct q4rdna_kv_attention_args {
+    int type;   /* q4rdna_type of q and out */
+    int tokens; /* rows of q and out */
+    int heads;  /* query heads, a multiple of kv_heads; head h reads kv head h * kv_heads / heads */
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    float scale; /* of q . k; 0: 1 / sqrt(head_dim) */
+    int window;  /* a token sees itself and the window - 1 tokens before it; 0: all of them */
+} q4rdna_kv_attention_args;
+
+/* Bytes of one tile / of the whole cache (0 for a bad shape). */
+size_t q4rdna_kv_tile_bytes(int head_dim);
+size_t q4rdna_kv_cache_bytes(const q4rdna_kv_cache *cache);
+
+/* Writes the rows' k and v into the cache, and the rotated q to q_out (when
+ * heads > 0).  Per row and head, in f32: k and q are multiplied by
+ * norm / sqrt(mean square + eps) (with norm weights), then each pair (a, b) is
+ * turned by position * inv_freq (the product and its range reduction in f64).
+ * The scale of a tile (keys and values apart) becomes
+ *   s = max(s_before, max |x| / 127)        (e4m3: / 448)
+ * over the call's tokens in it; s_before is the tile's scale when it already
+ * held tokens of this sequence (its first row is older than this call) and 0
+ * otherwise.  Where s grew, the older codes become round(code * s_before / s);
+ * the new ones are round(x / s), to nearest even.  Rows of a tile behind the
+ * last token keep their bytes.  A k or v that is not finite makes its tile's
+ * scale NaN (so that every row that sees the tile becomes NaN) until the tile
+ * is begun anew.  Two sequences of one call must not write the same tile. */
+q4rdna_status q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
+                               const q4rdna_kv_append_args *args, q4rdna_stream_t stream);
+
+/* out = softmax(scale * q k^T) v over the cached tokens that the row's token
+ * sees: those up to itself, at most `window` of them.  A row that sees nothing
+ * becomes 0; rows outside every sequence keep their values.  Accumulation in
+ * f32.  The workspace (q4rdna_kv_attention_workspace_bytes, 16-byte aligned)
+ * needs no initialisation and carries nothing from call to call; calls that
+ * may overlap on the GPU need one each. */
+q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
+                                  const q4rdna_kv_attention_args *args, void *workspace, size_t workspace_bytes,
+                                  q4rdna_stream_t stream);
+/* 0 for arguments that q4rdna_kv_attention refuses, too. */
+size_t q4rdna_kv_attention_workspace_bytes(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
+                                           const q4rdna_kv_attention_args *args);
+
+/* The numbers of `count` pages (page_list: int32 device array) as
+ * k, v [count][kv_heads][page_tokens][head_dim] of the given type: code times
+ * scale in f32, rounded once. */
+q4rdna_status q4rdna_kv_dequant(const q4rdna_kv_cache *cache, const int32_t *page_list, int count, int type, void *k,
+                                void *v, q4rdna_stream_t stream);
+
 /* ---- sidecar (the reference's .q4rdna container, byte layout unchanged) ----
  * Header 48 B, entries 96 B, data at data_offset (source/q4rdna.cu:26-50).
  * Validation follows source/q4rdna.cu:131-152.  The whole data region is
@@ -379,8 +496,12 @@ uint64_t q4rdna_registry_hits(const char *weight_name);
  * (y) are complete.  Bit 2: a wait inside the tensor-core tile kernel (B >= 8)
  * ran out (about 1 s) and the kernel stopped; the outputs of that launch are
  * invalid and the workspaces it used must be re-initialised
- * (q4rdna_workspace_init) or the plans re-created.  Bit 0 is no longer set by
- * any kernel.  0 = no fault; 0xffffffff = the flag could not be read.  No
+ * (q4rdna_workspace_init) or the plans re-created.  Bit 3: a cache operator
+ * (q4rdna_kv_*) met a page outside the cache, a length above max_length or a
+ * q_start outside the rows; what lies there was neither read nor written.
+ * Bit 4: a wait inside the attention's tensor-core kernel ran out (about 1 s);
+ * the outputs of that launch are invalid.  Bit 0 is no longer set by any
+ * kernel.  0 = no fault; 0xffffffff = the flag could not be read.  No
  * reference counterpart (the reference kernels never wait). */
 uint32_t q4rdna_take_fault(void);
 /* Prints the reference's exit-time summary to stderr (also run at exit once the

@@ -37,6 +37,7 @@
 #include <vector>
 
 #include "q4rdna.h"
+#include "q4rdna_kv.h"
 #include "q4rdna_q4k.h"
 #include "q4rdna_tile.h"
 
@@ -1645,7 +1646,8 @@ uint32_t q4rdna_take_fault(void) {
     unsigned v = 0, zero = 0;
     if (cudaMemcpyFromSymbol(&v, g_fault, sizeof(v)) != cudaSuccess) return 0xffffffffu;
     if (v != 0) cudaMemcpyToSymbol(g_fault, &zero, sizeof(zero));
-    return v;
+    const uint32_t kv = q4kv_take_fault();  // the cache operators' flags
+    return kv == 0xffffffffu ? kv : v | kv;
 }
 
 }  // extern "C"

@@ -27,6 +27,9 @@ OK = 0
 OP_PLAIN, OP_ADD, OP_SWIGLU = 0, 1, 2
 FORMAT_Q4RDNA, FORMAT_Q4K = 0, 1
 Q4K_BLOCK, Q4K_BLOCK_BYTES = 256, 144
+KV_INT8, KV_E4M3 = 0, 1
+KV_BLOCK = 16
+ROPE_NEOX, ROPE_NORM = 0, 1
 MAX_BATCH = 16
 STATUS = {
     0: "OK", 1: "INVALID_ARGUMENT", 2: "SHAPE", 3: "ALIGNMENT", 4: "WORKSPACE", 5: "UNSUPPORTED",
@@ -56,6 +59,29 @@ class GemvDesc(ctypes.Structure):
 class PlanInfo(ctypes.Structure):
     _fields_ = [("count", c_int), ("batch", c_int), ("items", c_int64), ("grid", c_int),
                 ("weight_bytes", c_uint64), ("algo_bytes", c_uint64), ("workspace_bytes", c_size_t)]
+
+
+class KVCacheDesc(ctypes.Structure):
+    _fields_ = [("tiles", c_void_p), ("pages", c_int), ("page_tokens", c_int), ("kv_heads", c_int),
+                ("head_dim", c_int), ("format", c_int)]
+
+
+class KVBatchDesc(ctypes.Structure):
+    _fields_ = [("page_table", c_void_p), ("lengths", c_void_p), ("q_start", c_void_p), ("sequences", c_int),
+                ("table_stride", c_int), ("max_length", c_int)]
+
+
+class KVAppendArgs(ctypes.Structure):
+    _fields_ = [("type", c_int), ("tokens", c_int), ("heads", c_int), ("k", c_void_p), ("v", c_void_p),
+                ("q", c_void_p), ("q_out", c_void_p), ("k_stride", c_int64), ("v_stride", c_int64),
+                ("q_stride", c_int64), ("q_out_stride", c_int64), ("inv_freq", c_void_p), ("rotary_dim", c_int),
+                ("rope", c_int), ("positions", c_void_p), ("q_norm", c_void_p), ("k_norm", c_void_p),
+                ("norm_eps", ctypes.c_float)]
+
+
+class KVAttentionArgs(ctypes.Structure):
+    _fields_ = [("type", c_int), ("tokens", c_int), ("heads", c_int), ("q", c_void_p), ("out", c_void_p),
+                ("q_stride", c_int64), ("out_stride", c_int64), ("scale", ctypes.c_float), ("window", c_int)]
 
 
 def _bind(lib):
@@ -92,6 +118,12 @@ def _bind(lib):
         "q4rdna_ipc_open": (c_int, [ctypes.c_char_p, POINTER(P)]),
         "q4rdna_ipc_close": (c_int, [P]),
         "q4rdna_ipc_free": (c_int, [P]),
+        "q4rdna_kv_tile_bytes": (c_size_t, [c_int]),
+        "q4rdna_kv_cache_bytes": (c_size_t, [P]),
+        "q4rdna_kv_append": (c_int, [P, P, P, P]),
+        "q4rdna_kv_attention": (c_int, [P, P, P, P, c_size_t, P]),
+        "q4rdna_kv_attention_workspace_bytes": (c_size_t, [P, P, P]),
+        "q4rdna_kv_dequant": (c_int, [P, P, c_int, c_int, P, P, P]),
         "q4rdna_sidecar_open": (c_int, [c_char_p, c_int, POINTER(P)]),
         "q4rdna_sidecar_close": (None, [P]),
         "q4rdna_sidecar_count": (c_int, [P]),
@@ -142,6 +174,8 @@ SYMBOLS = [
     "q4rdna_plan_run_host", "q4rdna_plan_set_segments", "q4rdna_plan_run_many", "q4rdna_plan_set_flags", "q4rdna_plan_set_gather", "q4rdna_plan_gather_parity",
     "q4rdna_plan_set_gather_timeout", "q4rdna_ipc_alloc", "q4rdna_ipc_open",
     "q4rdna_ipc_close", "q4rdna_ipc_free",
+    "q4rdna_kv_tile_bytes", "q4rdna_kv_cache_bytes", "q4rdna_kv_append", "q4rdna_kv_attention",
+    "q4rdna_kv_attention_workspace_bytes", "q4rdna_kv_dequant",
     "q4rdna_sidecar_open", "q4rdna_sidecar_close", "q4rdna_sidecar_count", "q4rdna_sidecar_entry",
     "q4rdna_sidecar_find", "q4rdna_mul_mat", "q4rdna_mul_mat_add", "q4rdna_mul_mat_glu",
     "q4rdna_launch_count", "q4rdna_take_fault", "q4rdna_registry_hits", "q4rdna_report_stats", "q4rdna_registry_reset",
@@ -420,6 +454,220 @@ def run_plans(plans, stream=None):
     (q4rdna_plan_run_many); each as Plan.run would."""
     arr = (c_void_p * len(plans))(*[p._h.value for p in plans])
     check(_lib().q4rdna_plan_run_many(arr, len(plans), _stream_handle(stream)), "plan_run_many")
+
+
+# ------------------------------------------------------ key/value cache
+
+class KVCache:
+    """A paged key/value cache in 8 bits (layout: include/q4rdna.h).
+
+    ``tiles``: uint8 CUDA tensor [pages, kv_heads, page_tokens / 16, 16 + 32 *
+    head_dim], allocated (zeroed) here unless given.  format KV_INT8 or KV_E4M3;
+    head_dim 64, 128 or 256; page_tokens 16, 32, 64, 128 or 256.
+    """
+
+    def __init__(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, format: int = KV_INT8,
+                 device="cuda", tiles=None):
+        import torch
+
+        self._desc = KVCacheDesc(None, pages, page_tokens, kv_heads, head_dim, format)
+        if format not in (KV_INT8, KV_E4M3):
+            raise ValueError(f"unknown cache format {format}")
+        nbytes = _lib().q4rdna_kv_cache_bytes(ctypes.byref(self._desc))
+        if nbytes == 0:
+            raise ValueError("kv cache: pages and kv_heads positive, page_tokens a power of two in [16, 256], "
+                             "head_dim 64, 128 or 256")
+        shape = (pages, kv_heads, page_tokens // KV_BLOCK, 16 + 32 * head_dim)
+        if tiles is None:
+            tiles = torch.zeros(shape, dtype=torch.uint8, device=device)
+        if tiles.dtype != torch.uint8 or not tiles.is_contiguous() or tiles.numel() != nbytes:
+            raise ValueError(f"kv cache tiles: a contiguous uint8 tensor of {nbytes} bytes")
+        self.tiles = tiles
+        self.page_tokens, self.kv_heads, self.head_dim, self.format = page_tokens, kv_heads, head_dim, format
+        self.device = tiles.device
+        self._desc.tiles = tiles.data_ptr()
+        self._ref = ctypes.byref(self._desc)
+
+
+class KVBatch:
+    """The sequences of a call: page_table int32 [sequences, pages of one], lengths
+    int32 [sequences] (the tokens of each with the call's own, the last ones) and
+    q_start int32 [sequences + 1] (rows of each; None: one row each).  CUDA
+    tensors, read when the kernels run: rewrite them in place between steps and
+    replays.  max_length bounds every length (0: the page table's width)."""
+
+    def __init__(self, page_table, lengths, q_start=None, max_length: int = 0):
+        import torch
+
+        for name, t in (("page_table", page_table), ("lengths", lengths), ("q_start", q_start)):
+            if t is not None and (t.dtype != torch.int32 or t.device != page_table.device):
+                raise ValueError(f"kv batch: {name} is int32, on the page table's device")
+        S = lengths.numel()
+        if page_table.dim() != 2 or page_table.shape[0] != S or page_table.shape[1] < 1 or (
+                page_table.stride(1) != 1 and page_table.shape[1] > 1):
+            raise ValueError("kv batch: page_table is [sequences, pages], a row contiguous")
+        if not lengths.is_contiguous() or (q_start is not None and (not q_start.is_contiguous() or
+                                                                    q_start.numel() != S + 1)):
+            raise ValueError("kv batch: lengths [sequences] and q_start [sequences + 1], contiguous")
+        if S > 1 and page_table.stride(0) < page_table.shape[1]:
+            raise ValueError("kv batch: the page table's rows overlap")
+        self._keep = (page_table, lengths, q_start)
+        self.device = page_table.device
+        self.sequences = S
+        # the rows' stride is the table's width for the library; only the last row may be shorter than it
+        stride = page_table.stride(0) if S > 1 else page_table.shape[1]
+        self.pages = page_table.shape[1]
+        self._limit = max_length
+        self._desc = KVBatchDesc(page_table.data_ptr(), lengths.data_ptr(),
+                                 None if q_start is None else q_start.data_ptr(), S, stride, max_length)
+        self._ref = ctypes.byref(self._desc)
+
+    def _for(self, cache):
+        """The descriptor for this cache's page size."""
+        room = self.pages * cache.page_tokens
+        if self._limit > room:
+            raise ValueError(f"kv batch: max_length {self._limit} is more than the page table's {room} tokens")
+        self._desc.max_length = self._limit if self._limit else min(room, 2 ** 31 - 1 - 256)
+        return self._ref
+
+
+_KV_TYPES = None
+
+
+def _kv_type(dtype) -> int:
+    global _KV_TYPES
+    if _KV_TYPES is None:
+        import torch
+
+        _KV_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    t = _KV_TYPES.get(dtype)
+    if t is None:
+        raise ValueError("kv cache operators take float32, float16 or bfloat16")
+    return t
+
+
+def _kv_rows(x, heads, cache, like=None):
+    """(heads, row stride in elements) of [rows, heads, head_dim] or [rows, heads * head_dim]."""
+    D = cache.head_dim
+    shape = x.shape
+    if x.device != cache.device or (like is not None and (x.dtype != like.dtype or shape[0] != like.shape[0])):
+        raise ValueError("kv cache operators: rows of one type and number, on the cache's device")
+    if len(shape) == 3:
+        st = x.stride()
+        n, packed = shape[1], shape[2] == D and st[2] == 1 and (st[1] == D or shape[1] == 1)
+    else:
+        st = x.stride() if len(shape) == 2 else (0, 0)
+        n, packed = shape[-1] // D, len(shape) == 2 and shape[1] % D == 0 and st[1] == 1
+    if not packed or (heads and n != heads):
+        raise ValueError(f"kv cache operators: rows are [rows, heads, {D}], the heads of a row contiguous")
+    return n, st[0] if shape[0] > 1 else n * D
+
+
+def _kv_on(fn, cache, stream, *args):
+    """fn(*args) with the cache's device and the given stream current."""
+    import torch
+
+    if stream is not None:
+        if stream.device != cache.device:
+            raise ValueError("kv cache operators: the stream is on another device than the cache")
+        with torch.cuda.stream(stream):
+            return fn(*args)
+    if cache.device.index != torch.cuda.current_device():
+        with torch.cuda.device(cache.device):
+            return fn(*args)
+    return fn(*args)
+
+
+def kv_append(cache: KVCache, batch: KVBatch, k, v, *, q=None, q_out=None, inv_freq=None, rotary_dim: int = 0,
+              rope: int = ROPE_NEOX, positions=None, q_norm=None, k_norm=None, norm_eps: float = 1e-6, stream=None):
+    """Writes the rows' keys and values into the cache (q4rdna_kv_append).
+
+    k, v [rows, kv_heads, head_dim] and q [rows, heads, head_dim] (f32, f16 or
+    bf16; rows may be strided).  q_norm / k_norm (f32 [head_dim]) apply the
+    per-head RMSNorm; inv_freq (f32 [rotary_dim / 2]) the rotation at positions
+    (int32 [rows]; None: the token's number).  Returns the rotated q (q_out, or a
+    new tensor), None without q.
+    """
+    return _kv_on(_kv_append, cache, stream, cache, batch, k, v, q, q_out, inv_freq, rotary_dim, rope, positions,
+                  q_norm, k_norm, norm_eps)
+
+
+def _kv_append(cache, batch, k, v, q, q_out, inv_freq, rotary_dim, rope, positions, q_norm, k_norm, norm_eps):
+    import torch
+
+    _, ks = _kv_rows(k, cache.kv_heads, cache)
+    _, vs = _kv_rows(v, cache.kv_heads, cache, k)
+    heads = qs = qos = 0
+    if q is not None:
+        heads, qs = _kv_rows(q, 0, cache, k)
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _, qos = _kv_rows(q_out, heads, cache, k)
+    elif q_out is not None:
+        raise ValueError("kv_append: q_out without q")
+    D = cache.head_dim
+    for name, t, dtype, n in (("inv_freq", inv_freq, torch.float32, (rotary_dim or D) // 2),
+                              ("positions", positions, torch.int32, k.shape[0]), ("q_norm", q_norm, torch.float32, D),
+                              ("k_norm", k_norm, torch.float32, D)):
+        if t is not None and (t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or t.numel() != n):
+            raise ValueError(f"kv_append: {name} is a contiguous {dtype} tensor of {n}, on the cache's device")
+    if batch.device != cache.device:
+        raise ValueError("kv_append: the batch is on another device than the cache")
+    a = KVAppendArgs(_kv_type(k.dtype), k.shape[0], heads, k.data_ptr(), v.data_ptr(),
+                     None if q is None else q.data_ptr(), None if q is None else q_out.data_ptr(), ks, vs, qs, qos,
+                     None if inv_freq is None else inv_freq.data_ptr(), rotary_dim, rope,
+                     None if positions is None else positions.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
+                     None if k_norm is None else k_norm.data_ptr(), norm_eps)
+    check(_lib().q4rdna_kv_append(cache._ref, batch._for(cache), ctypes.byref(a),
+                                  torch.cuda.current_stream().cuda_stream), "kv_append")
+    return q_out
+
+
+def kv_attention(cache: KVCache, batch: KVBatch, q, *, scale: float = 0.0, window: int = 0, out=None, stream=None):
+    """softmax(scale * q k^T) v over the cache (q4rdna_kv_attention): each row of
+    q [rows, heads, head_dim] sees its sequence's tokens up to itself, at most
+    `window` of them (0: all).  scale 0: 1 / sqrt(head_dim).  A row that sees
+    nothing becomes 0; rows outside every sequence are left as they were."""
+    return _kv_on(_kv_attention, cache, stream, cache, batch, q, scale, window, out)
+
+
+def _kv_attention(cache, batch, q, scale, window, out):
+    import torch
+
+    heads, qs = _kv_rows(q, 0, cache)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _, os_ = _kv_rows(out, heads, cache, q)
+    if batch.device != cache.device:
+        raise ValueError("kv_attention: the batch is on another device than the cache")
+    a = KVAttentionArgs(_kv_type(q.dtype), q.shape[0], heads, q.data_ptr(), out.data_ptr(), qs, os_, scale, window)
+    L, ref, b = _lib(), ctypes.byref(a), batch._for(cache)
+    n = L.q4rdna_kv_attention_workspace_bytes(cache._ref, b, ref)
+    # a workspace of its own for each call: calls on different streams and captured
+    # graphs (whose pool it then belongs to) share nothing
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    check(L.q4rdna_kv_attention(cache._ref, b, ref, ws.data_ptr() if n else None, n,
+                                torch.cuda.current_stream().cuda_stream), "kv_attention")
+    return out
+
+
+def kv_dequant(cache: KVCache, pages, *, dtype=None, stream=None):
+    """(k, v) of the listed pages (int32 CUDA tensor), each [len(pages), kv_heads,
+    page_tokens, head_dim] of dtype (float32 by default): q4rdna_kv_dequant."""
+    return _kv_on(_kv_dequant, cache, stream, cache, pages, dtype)
+
+
+def _kv_dequant(cache, pages, dtype):
+    import torch
+
+    dtype = torch.float32 if dtype is None else dtype
+    if pages.dtype != torch.int32 or not pages.is_contiguous() or pages.device != cache.device:
+        raise ValueError("kv_dequant: pages is a contiguous int32 tensor on the cache's device")
+    shape = (pages.numel(), cache.kv_heads, cache.page_tokens, cache.head_dim)
+    k, v = (torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
+    check(_lib().q4rdna_kv_dequant(cache._ref, pages.data_ptr(), shape[0], _kv_type(dtype), k.data_ptr(),
+                                   v.data_ptr(), torch.cuda.current_stream().cuda_stream), "kv_dequant")
+    return k, v
 
 
 class Sidecar:

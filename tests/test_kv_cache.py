@@ -1,0 +1,162 @@
+"""Refusals and host-side rules of the key/value cache operators.  No GPU: every
+check runs before the first CUDA call."""
+import ctypes
+
+import pytest
+import torch
+
+import q4rdna
+from q4rdna import KVAppendArgs, KVAttentionArgs, KVBatchDesc, KVCacheDesc
+
+A = 0x10000  # an aligned address that nothing reads
+
+
+def desc(**kw):
+    d = dict(tiles=A, pages=4, page_tokens=32, kv_heads=2, head_dim=128, format=0)
+    d.update(kw)
+    return KVCacheDesc(*d.values())
+
+
+def batch(**kw):
+    d = dict(page_table=A, lengths=A, q_start=None, sequences=3, table_stride=2, max_length=0)
+    d.update(kw)
+    return KVBatchDesc(*d.values())
+
+
+def append_args(**kw):
+    d = dict(type=0, tokens=3, heads=4, k=A, v=A, q=A, q_out=A, k_stride=256, v_stride=256, q_stride=512,
+             q_out_stride=512, inv_freq=A, rotary_dim=0, rope=0, positions=None, q_norm=None, k_norm=None,
+             norm_eps=1e-6)
+    d.update(kw)
+    return KVAppendArgs(*d.values())
+
+
+def attention_args(**kw):
+    d = dict(type=0, tokens=3, heads=4, q=A, out=A, q_stride=512, out_stride=512, scale=0.0, window=0)
+    d.update(kw)
+    return KVAttentionArgs(*d.values())
+
+
+def refs(*xs):
+    return [None if x is None else ctypes.byref(x) for x in xs]
+
+
+INVALID, SHAPE, ALIGNMENT, WORKSPACE, TOO_LARGE = 1, 2, 3, 4, 11
+
+CACHES = [(dict(tiles=None), INVALID), (dict(tiles=A + 8), ALIGNMENT), (dict(pages=0), INVALID),
+          (dict(kv_heads=-1), INVALID), (dict(page_tokens=8), SHAPE), (dict(page_tokens=48), SHAPE),
+          (dict(page_tokens=512), SHAPE), (dict(head_dim=96), SHAPE), (dict(head_dim=0), SHAPE),
+          (dict(format=2), INVALID)]
+BATCHES = [(dict(page_table=None), INVALID), (dict(lengths=None), INVALID), (dict(sequences=-1), INVALID),
+           (dict(sequences=2), SHAPE), (dict(table_stride=0), INVALID), (dict(max_length=65), SHAPE),
+           (dict(max_length=-1), INVALID)]
+
+
+@pytest.mark.parametrize("kw,status", CACHES)
+def test_cache_refusals(kw, status):
+    L = q4rdna.lib
+    c, b = refs(desc(**kw), batch())
+    assert L.q4rdna_kv_append(c, b, *refs(append_args()), None) == status
+    assert L.q4rdna_kv_attention(c, b, *refs(attention_args()), A, 1 << 30, None) == status
+    assert L.q4rdna_kv_attention_workspace_bytes(c, b, *refs(attention_args())) == 0
+    assert L.q4rdna_kv_dequant(c, A, 1, 0, A, A, None) == status
+
+
+@pytest.mark.parametrize("kw,status", BATCHES)
+def test_batch_refusals(kw, status):
+    L = q4rdna.lib
+    c, b = refs(desc(), batch(**kw))
+    assert L.q4rdna_kv_append(c, b, *refs(append_args()), None) == status
+    assert L.q4rdna_kv_attention(c, b, *refs(attention_args()), A, 1 << 30, None) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(type=3), INVALID), (dict(heads=-2), INVALID), (dict(rope=2), INVALID), (dict(heads=3), SHAPE),
+    (dict(k=None), INVALID), (dict(v=None), INVALID), (dict(q=None), INVALID), (dict(q_out=None), INVALID),
+    (dict(k=A + 4), ALIGNMENT), (dict(q_out=A + 8), ALIGNMENT), (dict(k_stride=255), SHAPE),
+    (dict(v_stride=258), ALIGNMENT), (dict(type=1, q_stride=516), ALIGNMENT), (dict(q_stride=511), SHAPE),
+    (dict(rotary_dim=24), SHAPE), (dict(rotary_dim=144), SHAPE), (dict(rotary_dim=-16), SHAPE),
+    (dict(k_norm=A + 4), ALIGNMENT), (dict(tokens=-1), INVALID), (dict(q_norm=A, norm_eps=-1e-6), INVALID),
+    (dict(k_norm=A, norm_eps=float("nan")), INVALID)])
+def test_append_refusals(kw, status):
+    c, b = refs(desc(), batch())
+    assert q4rdna.lib.q4rdna_kv_append(c, b, *refs(append_args(**kw)), None) == status
+    assert q4rdna.lib.q4rdna_kv_append(c, b, None, None) == INVALID
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(type=-1), INVALID), (dict(heads=0), INVALID), (dict(heads=5), SHAPE), (dict(q=None), INVALID),
+    (dict(out=None), INVALID), (dict(out=A + 2), ALIGNMENT), (dict(q_stride=500), SHAPE),
+    (dict(out_stride=513), ALIGNMENT), (dict(window=-1), INVALID), (dict(scale=-1.0), INVALID),
+    (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID)])
+def test_attention_refusals(kw, status):
+    c, b = refs(desc(), batch())
+    args = refs(attention_args(**kw))
+    assert q4rdna.lib.q4rdna_kv_attention(c, b, *args, A, 1 << 30, None) == status
+    assert q4rdna.lib.q4rdna_kv_attention_workspace_bytes(c, b, *args) == 0
+    assert q4rdna.lib.q4rdna_kv_attention(c, b, None, A, 1 << 30, None) == INVALID
+
+
+def test_too_many_rows_are_refused():
+    n = (1 << 28) + 1
+    c, b = refs(desc(), batch(sequences=n))
+    assert q4rdna.lib.q4rdna_kv_append(c, b, *refs(append_args(tokens=n)), None) == TOO_LARGE
+    assert q4rdna.lib.q4rdna_kv_attention(c, b, *refs(attention_args(tokens=n)), A, 1 << 40, None) == TOO_LARGE
+
+
+def test_dequant_refusals():
+    c, = refs(desc())
+    f = q4rdna.lib.q4rdna_kv_dequant
+    assert f(c, A, -1, 0, A, A, None) == INVALID
+    assert f(c, A, 1, 3, A, A, None) == INVALID
+    assert f(c, None, 1, 0, A, A, None) == INVALID
+    assert f(c, A, 1, 0, A + 4, A, None) == ALIGNMENT
+    assert f(c, A, 1 << 30, 0, A, A, None) == TOO_LARGE
+
+
+def test_nothing_to_do_is_ok():
+    c, b = refs(desc(), batch(sequences=0))
+    none = dict(tokens=0, k=None, v=None, q=None, q_out=None)
+    assert q4rdna.lib.q4rdna_kv_append(c, b, *refs(append_args(**none)), None) == 0
+    assert q4rdna.lib.q4rdna_kv_attention(c, b, *refs(attention_args(tokens=0, q=None, out=None)), None, 0, None) == 0
+    assert q4rdna.lib.q4rdna_kv_dequant(c, None, 0, 0, None, None, None) == 0
+
+
+def test_sizes():
+    assert q4rdna.lib.q4rdna_kv_tile_bytes(128) == 16 + 2 * 16 * 128
+    assert q4rdna.lib.q4rdna_kv_tile_bytes(80) == 0
+    assert q4rdna.lib.q4rdna_kv_cache_bytes(ctypes.byref(desc())) == 4 * 2 * 2 * (16 + 32 * 128)
+    big = desc(pages=1 << 20, page_tokens=256, kv_heads=8)
+    assert q4rdna.lib.q4rdna_kv_cache_bytes(ctypes.byref(big)) == (1 << 20) * 8 * 16 * 4112  # past 32 bits
+
+
+def test_python_refusals():
+    cache = q4rdna.KVCache(4, 16, 2, 64, device="cpu")
+    assert cache.tiles.shape == (4, 2, 1, 16 + 32 * 64)
+    with pytest.raises(ValueError):
+        q4rdna.KVCache(4, 24, 2, 64, device="cpu")
+    with pytest.raises(ValueError):
+        q4rdna.KVCache(4, 16, 2, 64, format=7, device="cpu")
+    with pytest.raises(ValueError):
+        q4rdna.KVCache(4, 16, 2, 64, tiles=cache.tiles[:3])
+    i32 = dict(dtype=torch.int32)
+    table, lengths = torch.zeros((3, 2), **i32), torch.zeros(3, **i32)
+    for bad in [(table.long(), lengths), (table, lengths.long()), (table[:2], lengths), (table[:, ::2], lengths[:2]),
+                (table.expand(3, 2)[:1].expand(3, 2), lengths), (table, lengths, torch.zeros(3, **i32))]:
+        with pytest.raises(ValueError):
+            q4rdna.KVBatch(*bad)
+    wide = torch.zeros((3, 5), **i32)[:, :2]  # rows of a wider table
+    assert q4rdna.KVBatch(wide, lengths)._desc.table_stride == 5
+    with pytest.raises(ValueError):
+        q4rdna.KVBatch(table, lengths, max_length=33)._for(cache)
+    x = torch.zeros((3, 2, 64))
+    for rows, heads in [(x[..., :32], 0), (x.transpose(0, 1), 3), (x.flatten(), 0), (x, 3),
+                        (torch.zeros((3, 2, 128))[..., ::2], 0), (torch.zeros((3, 4, 64))[:, ::2], 0)]:
+        with pytest.raises(ValueError):
+            q4rdna._kv_rows(rows, heads, cache)
+    assert q4rdna._kv_rows(x, 2, cache) == (2, 128)
+    assert q4rdna._kv_rows(torch.zeros((3, 512))[:, 128:256], 2, cache) == (2, 512)  # a part of fused rows
+    with pytest.raises(ValueError):
+        q4rdna._kv_rows(x.bfloat16(), 2, cache, x)
+    with pytest.raises(ValueError):
+        q4rdna._kv_type(torch.float64)
