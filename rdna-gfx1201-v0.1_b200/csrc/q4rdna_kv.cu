@@ -4,6 +4,8 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
+#include <map>
+#include <mutex>
 
 #include "q4rdna_kv.h"
 #include "q4rdna_kv_append.cuh"
@@ -63,6 +65,29 @@ q4rdna_status check_rows(const void *p, int64_t stride, int type, int heads, int
 
 bool known_type(int t) { return t == Q4RDNA_F32 || t == Q4RDNA_F16 || t == Q4RDNA_BF16; }
 
+// One launch as a programmatic dependent of the stream's last kernel: it may be
+// set up while that one ends, and every kernel here waits for it
+// (griddepcontrol.wait) before its first access.
+template <class Args>
+q4rdna_status launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args &args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, args) != cudaSuccess) {
+        cudaGetLastError();
+        return Q4RDNA_ERR_CUDA;
+    }
+    q4::g_launches.fetch_add(1, std::memory_order_relaxed);
+    return Q4RDNA_OK;
+}
+
 q4rdna_status launched() {
     if (cudaGetLastError() != cudaSuccess) return Q4RDNA_ERR_CUDA;
     q4::g_launches.fetch_add(1, std::memory_order_relaxed);
@@ -93,6 +118,79 @@ q4rdna_status check_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_batc
     const float scale = args->scale > 0.0f ? args->scale : 1.0f / std::sqrt((float)D);
     A.scale = scale * 1.44269504088896340736f;
     A.window = args->window;
+    return Q4RDNA_OK;
+}
+
+// ---- the attention's launches
+
+using AttnKernel = void (*)(AttnArgs);
+
+struct Variant {
+    AttnKernel split, join;
+    size_t smem;
+};
+
+template <int D, int FMT, int NT, int TERMS>
+Variant variant() {
+    return {kv_attention_kernel<D, FMT, NT, TERMS>, kv_join_kernel<D, 8 * NT>, sizeof(AttnSmem<D, NT>)};
+}
+template <int D, int FMT>
+Variant variant(int nt, int terms) {
+    if (nt == 1) return terms == 1 ? variant<D, FMT, 1, 1>() : variant<D, FMT, 1, 2>();
+    return terms == 1 ? variant<D, FMT, 2, 1>() : variant<D, FMT, 2, 2>();
+}
+template <int D>
+Variant variant(int format, int nt, int terms) {
+    return format == Q4RDNA_KV_INT8 ? variant<D, Q4RDNA_KV_INT8>(nt, terms) : variant<D, Q4RDNA_KV_E4M3>(nt, terms);
+}
+
+struct AttnLaunch {
+    AttnKernel split, join;
+    int nc;            // columns of a task
+    unsigned grid;     // CTAs, one share each
+    size_t smem, workspace;
+};
+
+// CTAs of the split kernel that the current device holds at once (and its
+// shared-memory limit raised); 0 on an error
+int resident_ctas(const Variant &v) {
+    static std::mutex mu;
+    static std::map<std::pair<int, AttnKernel>, int> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    std::lock_guard<std::mutex> lock(mu);
+    int &n = known[{dev, v.split}];
+    if (n == 0) {
+        int sms = 0, occ = 0;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+            cudaFuncSetAttribute(v.split, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, v.split, kAttnThreads, v.smem) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        n = sms * std::max(occ, 1);
+    }
+    return n;
+}
+
+q4rdna_status plan_attention(AttnArgs &A, int D, AttnLaunch &L) {
+    // one column tile where a token's heads fit it and each sequence has one token, else two
+    const int nt = A.b.q_start == nullptr && A.group <= 8 ? 1 : 2;
+    const int terms = A.type == Q4RDNA_F32 ? 2 : 1;
+    const Variant v = D == 64 ? variant<64>(A.c.format, nt, terms)
+                              : D == 128 ? variant<128>(A.c.format, nt, terms) : variant<256>(A.c.format, nt, terms);
+    const int ctas = resident_ctas(v);
+    if (ctas == 0) return Q4RDNA_ERR_DEVICE;
+    L.split = v.split;
+    L.join = v.join;
+    L.smem = v.smem;
+    L.nc = 8 * nt;
+    A.min_share = kAttnWarps;  // one block per warp
+    // no more CTAs than the largest work has shares
+    const double tasks = ((double)A.b.T * A.group / L.nc + A.b.S) * A.c.hk;
+    const double work = tasks * (A.b.max_len / kBlock + 1);
+    L.grid = (unsigned)std::max(1.0, std::min((double)ctas, work / A.min_share + 1.0));
+    L.workspace = (size_t)L.grid * (2 * sizeof(int4) + 2 * sizeof(float) * part_floats(D, L.nc));
     return Q4RDNA_OK;
 }
 
@@ -151,11 +249,8 @@ q4rdna_status q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_bat
     A.eps = args->norm_eps;
     const int units = batch->q_start == nullptr ? batch->sequences : args->tokens / kBlock + 2 * batch->sequences;
     const dim3 grid((unsigned)units, (unsigned)std::min(cache->kv_heads, 65535));
-    const cudaStream_t cs = (cudaStream_t)stream;
-    if (D == 64) kv_append_kernel<64><<<grid, kAppendThreads, 0, cs>>>(A);
-    else if (D == 128) kv_append_kernel<128><<<grid, kAppendThreads, 0, cs>>>(A);
-    else kv_append_kernel<256><<<grid, kAppendThreads, 0, cs>>>(A);
-    return launched();
+    return launch(D == 64 ? kv_append_kernel<64> : D == 128 ? kv_append_kernel<128> : kv_append_kernel<256>, grid,
+                  kAppendThreads, 0, (cudaStream_t)stream, A);
 }
 
 q4rdna_status q4rdna_kv_dequant(const q4rdna_kv_cache *cache, const int32_t *page_list, int count, int type, void *k,
@@ -179,9 +274,11 @@ q4rdna_status q4rdna_kv_dequant(const q4rdna_kv_cache *cache, const int32_t *pag
 
 size_t q4rdna_kv_attention_workspace_bytes(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
                                            const q4rdna_kv_attention_args *args) {
-    q4kv::AttnArgs A{};
-    if (q4kv::check_attention(cache, batch, args, A) != Q4RDNA_OK) return 0;
-    return 0;
+    using namespace q4kv;
+    AttnArgs A{};
+    AttnLaunch L;
+    if (check_attention(cache, batch, args, A) != Q4RDNA_OK || args->tokens == 0 || batch->sequences == 0) return 0;
+    return plan_attention(A, cache->head_dim, L) == Q4RDNA_OK ? L.workspace : 0;
 }
 
 q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
@@ -189,18 +286,18 @@ q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_
                                   q4rdna_stream_t stream) {
     using namespace q4kv;
     AttnArgs A{};
-    const q4rdna_status st = check_attention(cache, batch, args, A);
+    AttnLaunch L;
+    q4rdna_status st = check_attention(cache, batch, args, A);
     if (st != Q4RDNA_OK) return st;
-    (void)workspace;
-    (void)workspace_bytes;
     if (args->tokens == 0 || batch->sequences == 0) return Q4RDNA_OK;
-    const long long n = ((long long)args->tokens * args->heads + 3) / 4;
-    if (n > 0x7fffffffLL) return Q4RDNA_ERR_TOO_LARGE;
+    if ((st = plan_attention(A, cache->head_dim, L)) != Q4RDNA_OK) return st;
+    if (workspace == nullptr || workspace_bytes < L.workspace) return Q4RDNA_ERR_WORKSPACE;
+    if (!aligned(workspace)) return Q4RDNA_ERR_ALIGNMENT;
+    A.rec = reinterpret_cast<int4 *>(workspace);
+    A.part = reinterpret_cast<float *>(A.rec + 2 * L.grid);
     const cudaStream_t cs = (cudaStream_t)stream;
-    if (cache->head_dim == 64) kv_attention_row_kernel<64><<<(unsigned)n, 128, 0, cs>>>(A);
-    else if (cache->head_dim == 128) kv_attention_row_kernel<128><<<(unsigned)n, 128, 0, cs>>>(A);
-    else kv_attention_row_kernel<256><<<(unsigned)n, 128, 0, cs>>>(A);
-    return launched();
+    if ((st = launch(L.split, dim3(L.grid), kAttnThreads, L.smem, cs, A)) != Q4RDNA_OK) return st;
+    return launch(L.join, dim3(L.grid), 32 * L.nc, 0, cs, A);
 }
 
 }  // extern "C"

@@ -170,11 +170,17 @@ __device__ __forceinline__ void load_codes(const uint8_t *p, int format, float (
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = from_code((uint32_t)(w >> (8 * i)) & 0xffu, format);
 }
+// x / (sc + low) to codes: the product with inv ~ 1 / sc, corrected by its remainder,
+// so that a quotient half-way between two codes is met exactly
 template <int N>
-__device__ __forceinline__ void store_codes(uint8_t *p, int format, const float (&x)[N], float inv) {
+__device__ __forceinline__ void store_codes(uint8_t *p, int format, const float (&x)[N], float sc, float low, float inv) {
     uint64_t w = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) w |= (uint64_t)to_code(x[i] * inv, format) << (8 * i);
+    for (int i = 0; i < N; ++i) {
+        const float y = x[i] * inv;
+        const float r = fmaf(-y, low, fmaf(-y, sc, x[i]));
+        w |= (uint64_t)to_code(fmaf(r, inv, y), format) << (8 * i);
+    }
     if constexpr (N == 2) *reinterpret_cast<uint16_t *>(p) = (uint16_t)w;
     else if constexpr (N == 4) *reinterpret_cast<uint32_t *>(p) = (uint32_t)w;
     else *reinterpret_cast<uint64_t *>(p) = w;

@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
     __shared__ uint32_t wmax[2][kAppendWarps][2];
     const Batch &B = A.b;
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     int s = blockIdx.x;
     if (B.q_start != nullptr) {  // the last sequence whose first unit is not behind this one
         int lo = 0, hi = B.S - 1;
@@ -155,17 +157,20 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             if (r0 > 0) old = *reinterpret_cast<const float2 *>(tile);
             __syncthreads();
             const float s_old[2] = {old.x, old.y};
-            float sc[2], inv[2];
+            float sc[2], low[2], inv[2];
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
                 uint32_t m = 0;
 #pragma unroll
                 for (int i = 0; i < kAppendWarps; ++i) m = max(m, wmax[par][i][z]);
-                float x = fmaxf(s_old[z], __uint_as_float(m) / top);
+                const float now = __uint_as_float(m) / top;
+                float x = fmaxf(s_old[z], now);
                 if (x < kTinyScale) x = 0.0f;
                 if (m >= 0x7f800000u || isnan(s_old[z])) x = __int_as_float(0x7fffffff);
                 sc[z] = x;
                 inv[z] = x > 0.0f ? 1.0f / x : 0.0f;
+                // what the rounding of max / top left out: 16-bit inputs give many exact halves of a step
+                low[z] = x > s_old[z] && x > 0.0f ? fmaf(-now, top, __uint_as_float(m)) / top : 0.0f;
             }
             if (threadIdx.x == 0) *reinterpret_cast<float2 *>(tile) = make_float2(sc[0], sc[1]);
 #pragma unroll
@@ -175,12 +180,14 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
                     for (int r = w; r < r0; r += kAppendWarps) {
                         float x[EPL];
                         load_codes<EPL>(codes + r * D, A.c.format, x);
-                        store_codes<EPL>(codes + r * D, A.c.format, x, s_old[z] * inv[z]);
+                        #pragma unroll
+                        for (int t = 0; t < EPL; ++t) x[t] *= s_old[z];
+                        store_codes<EPL>(codes + r * D, A.c.format, x, sc[z], low[z], inv[z]);
                     }
 #pragma unroll
                 for (int u = 0; u < kAppendRows; ++u) {
                     const int i = w + u * kAppendWarps;
-                    if (i < cnt) store_codes<EPL>(codes + (r0 + i) * D, A.c.format, z == 0 ? k[u] : v[u], inv[z]);
+                    if (i < cnt) store_codes<EPL>(codes + (r0 + i) * D, A.c.format, z == 0 ? k[u] : v[u], sc[z], low[z], inv[z]);
                 }
             }
         }
