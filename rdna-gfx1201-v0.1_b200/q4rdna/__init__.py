@@ -458,6 +458,35 @@ def run_plans(plans, stream=None):
 
 # ------------------------------------------------------ key/value cache
 
+class _KVCacheRec(ctypes.Structure):  # CacheRec of csrc/q4rdna_kv_torch.cpp
+    _fields_ = [("desc", KVCacheDesc), ("device", c_int)]
+
+
+class _KVBatchRec(ctypes.Structure):  # BatchRec of csrc/q4rdna_kv_torch.cpp
+    _fields_ = [("desc", KVBatchDesc), ("pages", c_int), ("limit", c_int), ("device", c_int)]
+
+
+_kv_module = None
+
+
+def _kv():
+    """The cache operators' call path (csrc/q4rdna_kv_torch.cpp), loaded on first use."""
+    global _kv_module
+    if _kv_module is None:
+        _lib()
+        import torch  # noqa: F401  (its libraries come first)
+
+        from . import _kv_torch
+
+        _kv_torch.set_check(check)
+        _kv_module = _kv_torch
+    return _kv_module
+
+
+def _device_index(t) -> int:
+    return t.device.index if t.is_cuda else -1
+
+
 class KVCache:
     """A paged key/value cache in 8 bits (layout: include/q4rdna.h).
 
@@ -470,10 +499,10 @@ class KVCache:
                  device="cuda", tiles=None):
         import torch
 
-        self._desc = KVCacheDesc(None, pages, page_tokens, kv_heads, head_dim, format)
+        desc = KVCacheDesc(None, pages, page_tokens, kv_heads, head_dim, format)
         if format not in (KV_INT8, KV_E4M3):
             raise ValueError(f"unknown cache format {format}")
-        nbytes = _lib().q4rdna_kv_cache_bytes(ctypes.byref(self._desc))
+        nbytes = _lib().q4rdna_kv_cache_bytes(ctypes.byref(desc))
         if nbytes == 0:
             raise ValueError("kv cache: pages and kv_heads positive, page_tokens a power of two in [16, 256], "
                              "head_dim 64, 128 or 256")
@@ -482,11 +511,13 @@ class KVCache:
             tiles = torch.zeros(shape, dtype=torch.uint8, device=device)
         if tiles.dtype != torch.uint8 or not tiles.is_contiguous() or tiles.numel() != nbytes:
             raise ValueError(f"kv cache tiles: a contiguous uint8 tensor of {nbytes} bytes")
+        desc.tiles = tiles.data_ptr()
         self.tiles = tiles
-        self.page_tokens, self.kv_heads, self.head_dim, self.format = page_tokens, kv_heads, head_dim, format
+        self.pages, self.page_tokens, self.kv_heads, self.head_dim = pages, page_tokens, kv_heads, head_dim
+        self.format = format
         self.device = tiles.device
-        self._desc.tiles = tiles.data_ptr()
-        self._ref = ctypes.byref(self._desc)
+        self._rec = _KVCacheRec(desc, _device_index(tiles))
+        self._at = ctypes.addressof(self._rec)
 
 
 class KVBatch:
@@ -511,71 +542,25 @@ class KVBatch:
             raise ValueError("kv batch: lengths [sequences] and q_start [sequences + 1], contiguous")
         if S > 1 and page_table.stride(0) < page_table.shape[1]:
             raise ValueError("kv batch: the page table's rows overlap")
+        if max_length < 0:
+            raise ValueError("kv batch: max_length is not negative")
         self._keep = (page_table, lengths, q_start)
         self.device = page_table.device
         self.sequences = S
-        # the rows' stride is the table's width for the library; only the last row may be shorter than it
-        stride = page_table.stride(0) if S > 1 else page_table.shape[1]
-        self.pages = page_table.shape[1]
-        self._limit = max_length
-        self._desc = KVBatchDesc(page_table.data_ptr(), lengths.data_ptr(),
-                                 None if q_start is None else q_start.data_ptr(), S, stride, max_length)
-        self._ref = ctypes.byref(self._desc)
-
-    def _for(self, cache):
-        """The descriptor for this cache's page size."""
-        room = self.pages * cache.page_tokens
-        if self._limit > room:
-            raise ValueError(f"kv batch: max_length {self._limit} is more than the page table's {room} tokens")
-        self._desc.max_length = self._limit if self._limit else min(room, 2 ** 31 - 1 - 256)
-        return self._ref
+        desc = KVBatchDesc(page_table.data_ptr(), lengths.data_ptr(), None if q_start is None else q_start.data_ptr(),
+                           S, page_table.stride(0) if S > 1 else page_table.shape[1], 0)
+        self._rec = _KVBatchRec(desc, page_table.shape[1], max_length, _device_index(page_table))
+        self._at = ctypes.addressof(self._rec)
 
 
-_KV_TYPES = None
-
-
-def _kv_type(dtype) -> int:
-    global _KV_TYPES
-    if _KV_TYPES is None:
-        import torch
-
-        _KV_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    t = _KV_TYPES.get(dtype)
-    if t is None:
-        raise ValueError("kv cache operators take float32, float16 or bfloat16")
-    return t
-
-
-def _kv_rows(x, heads, cache, like=None):
-    """(heads, row stride in elements) of [rows, heads, head_dim] or [rows, heads * head_dim]."""
-    D = cache.head_dim
-    shape = x.shape
-    if x.device != cache.device or (like is not None and (x.dtype != like.dtype or shape[0] != like.shape[0])):
-        raise ValueError("kv cache operators: rows of one type and number, on the cache's device")
-    if len(shape) == 3:
-        st = x.stride()
-        n, packed = shape[1], shape[2] == D and st[2] == 1 and (st[1] == D or shape[1] == 1)
-    else:
-        st = x.stride() if len(shape) == 2 else (0, 0)
-        n, packed = shape[-1] // D, len(shape) == 2 and shape[1] % D == 0 and st[1] == 1
-    if not packed or (heads and n != heads):
-        raise ValueError(f"kv cache operators: rows are [rows, heads, {D}], the heads of a row contiguous")
-    return n, st[0] if shape[0] > 1 else n * D
-
-
-def _kv_on(fn, cache, stream, *args):
-    """fn(*args) with the cache's device and the given stream current."""
+def _kv_on(stream, cache, fn, *args):
+    """fn(*args) on a stream that need not be the current one."""
     import torch
 
-    if stream is not None:
-        if stream.device != cache.device:
-            raise ValueError("kv cache operators: the stream is on another device than the cache")
-        with torch.cuda.stream(stream):
-            return fn(*args)
-    if cache.device.index != torch.cuda.current_device():
-        with torch.cuda.device(cache.device):
-            return fn(*args)
-    return fn(*args)
+    if stream.device != cache.device:
+        raise ValueError("kv cache operators: the stream is on another device than the cache")
+    with torch.cuda.stream(stream):
+        return fn(*args)
 
 
 def kv_append(cache: KVCache, batch: KVBatch, k, v, *, q=None, q_out=None, inv_freq=None, rotary_dim: int = 0,
@@ -588,39 +573,9 @@ def kv_append(cache: KVCache, batch: KVBatch, k, v, *, q=None, q_out=None, inv_f
     (int32 [rows]; None: the token's number).  Returns the rotated q (q_out, or a
     new tensor), None without q.
     """
-    return _kv_on(_kv_append, cache, stream, cache, batch, k, v, q, q_out, inv_freq, rotary_dim, rope, positions,
-                  q_norm, k_norm, norm_eps)
-
-
-def _kv_append(cache, batch, k, v, q, q_out, inv_freq, rotary_dim, rope, positions, q_norm, k_norm, norm_eps):
-    import torch
-
-    _, ks = _kv_rows(k, cache.kv_heads, cache)
-    _, vs = _kv_rows(v, cache.kv_heads, cache, k)
-    heads = qs = qos = 0
-    if q is not None:
-        heads, qs = _kv_rows(q, 0, cache, k)
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _, qos = _kv_rows(q_out, heads, cache, k)
-    elif q_out is not None:
-        raise ValueError("kv_append: q_out without q")
-    D = cache.head_dim
-    for name, t, dtype, n in (("inv_freq", inv_freq, torch.float32, (rotary_dim or D) // 2),
-                              ("positions", positions, torch.int32, k.shape[0]), ("q_norm", q_norm, torch.float32, D),
-                              ("k_norm", k_norm, torch.float32, D)):
-        if t is not None and (t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or t.numel() != n):
-            raise ValueError(f"kv_append: {name} is a contiguous {dtype} tensor of {n}, on the cache's device")
-    if batch.device != cache.device:
-        raise ValueError("kv_append: the batch is on another device than the cache")
-    a = KVAppendArgs(_kv_type(k.dtype), k.shape[0], heads, k.data_ptr(), v.data_ptr(),
-                     None if q is None else q.data_ptr(), None if q is None else q_out.data_ptr(), ks, vs, qs, qos,
-                     None if inv_freq is None else inv_freq.data_ptr(), rotary_dim, rope,
-                     None if positions is None else positions.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
-                     None if k_norm is None else k_norm.data_ptr(), norm_eps)
-    check(_lib().q4rdna_kv_append(cache._ref, batch._for(cache), ctypes.byref(a),
-                                  torch.cuda.current_stream().cuda_stream), "kv_append")
-    return q_out
+    f = (_kv_module or _kv()).append
+    a = (cache._at, batch._at, k, v, q, q_out, inv_freq, rotary_dim, rope, positions, q_norm, k_norm, norm_eps)
+    return f(*a) if stream is None else _kv_on(stream, cache, f, *a)
 
 
 def kv_attention(cache: KVCache, batch: KVBatch, q, *, scale: float = 0.0, window: int = 0, out=None, stream=None):
@@ -628,46 +583,21 @@ def kv_attention(cache: KVCache, batch: KVBatch, q, *, scale: float = 0.0, windo
     q [rows, heads, head_dim] sees its sequence's tokens up to itself, at most
     `window` of them (0: all).  scale 0: 1 / sqrt(head_dim).  A row that sees
     nothing becomes 0; rows outside every sequence are left as they were."""
-    return _kv_on(_kv_attention, cache, stream, cache, batch, q, scale, window, out)
-
-
-def _kv_attention(cache, batch, q, scale, window, out):
-    import torch
-
-    heads, qs = _kv_rows(q, 0, cache)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _, os_ = _kv_rows(out, heads, cache, q)
-    if batch.device != cache.device:
-        raise ValueError("kv_attention: the batch is on another device than the cache")
-    a = KVAttentionArgs(_kv_type(q.dtype), q.shape[0], heads, q.data_ptr(), out.data_ptr(), qs, os_, scale, window)
-    L, ref, b = _lib(), ctypes.byref(a), batch._for(cache)
-    n = L.q4rdna_kv_attention_workspace_bytes(cache._ref, b, ref)
-    # a workspace of its own for each call: calls on different streams and captured
-    # graphs (whose pool it then belongs to) share nothing
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    check(L.q4rdna_kv_attention(cache._ref, b, ref, ws.data_ptr() if n else None, n,
-                                torch.cuda.current_stream().cuda_stream), "kv_attention")
-    return out
+    f = (_kv_module or _kv()).attention
+    if stream is None:
+        return f(cache._at, batch._at, q, scale, window, out)
+    return _kv_on(stream, cache, f, cache._at, batch._at, q, scale, window, out)
 
 
 def kv_dequant(cache: KVCache, pages, *, dtype=None, stream=None):
     """(k, v) of the listed pages (int32 CUDA tensor), each [len(pages), kv_heads,
     page_tokens, head_dim] of dtype (float32 by default): q4rdna_kv_dequant."""
-    return _kv_on(_kv_dequant, cache, stream, cache, pages, dtype)
+    if dtype is None:
+        import torch
 
-
-def _kv_dequant(cache, pages, dtype):
-    import torch
-
-    dtype = torch.float32 if dtype is None else dtype
-    if pages.dtype != torch.int32 or not pages.is_contiguous() or pages.device != cache.device:
-        raise ValueError("kv_dequant: pages is a contiguous int32 tensor on the cache's device")
-    shape = (pages.numel(), cache.kv_heads, cache.page_tokens, cache.head_dim)
-    k, v = (torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
-    check(_lib().q4rdna_kv_dequant(cache._ref, pages.data_ptr(), shape[0], _kv_type(dtype), k.data_ptr(),
-                                   v.data_ptr(), torch.cuda.current_stream().cuda_stream), "kv_dequant")
-    return k, v
+        dtype = torch.float32
+    f = _kv().dequant
+    return f(cache._at, pages, dtype) if stream is None else _kv_on(stream, cache, f, cache._at, pages, dtype)
 
 
 class Sidecar:

@@ -146,17 +146,32 @@ def test_python_refusals():
         with pytest.raises(ValueError):
             q4rdna.KVBatch(*bad)
     wide = torch.zeros((3, 5), **i32)[:, :2]  # rows of a wider table
-    assert q4rdna.KVBatch(wide, lengths)._desc.table_stride == 5
+    rec = q4rdna.KVBatch(wide, lengths)._rec
+    assert rec.desc.table_stride == 5 and rec.pages == 2
     with pytest.raises(ValueError):
-        q4rdna.KVBatch(table, lengths, max_length=33)._for(cache)
-    x = torch.zeros((3, 2, 64))
-    for rows, heads in [(x[..., :32], 0), (x.transpose(0, 1), 3), (x.flatten(), 0), (x, 3),
-                        (torch.zeros((3, 2, 128))[..., ::2], 0), (torch.zeros((3, 4, 64))[:, ::2], 0)]:
+        q4rdna.KVBatch(table, lengths, max_length=-1)
+    x, batch = torch.zeros((3, 2, 64)), q4rdna.KVBatch(table, lengths)
+    with pytest.raises(ValueError, match="max_length"):
+        q4rdna.kv_attention(cache, q4rdna.KVBatch(table, lengths, max_length=33), x)
+    for bad in [x[..., :32], x.transpose(0, 2), x.flatten(), torch.zeros((3, 2, 128))[..., ::2],
+                torch.zeros((3, 4, 64))[:, ::2], torch.zeros((3, 100)), x.double(), None, 7, x]:
+        with pytest.raises(ValueError):  # the last one for its device
+            q4rdna.kv_attention(cache, batch, bad)
         with pytest.raises(ValueError):
-            q4rdna._kv_rows(rows, heads, cache)
-    assert q4rdna._kv_rows(x, 2, cache) == (2, 128)
-    assert q4rdna._kv_rows(torch.zeros((3, 512))[:, 128:256], 2, cache) == (2, 512)  # a part of fused rows
+            q4rdna.kv_append(cache, batch, bad, x)
+        with pytest.raises(ValueError):
+            q4rdna.kv_append(cache, batch, x, bad)
     with pytest.raises(ValueError):
-        q4rdna._kv_rows(x.bfloat16(), 2, cache, x)
+        q4rdna.kv_dequant(cache, table)
     with pytest.raises(ValueError):
-        q4rdna._kv_type(torch.float64)
+        q4rdna.kv_dequant(cache, table, dtype="float32")
+
+
+def test_python_refusals_by_shape_come_before_the_device():
+    """Messages name the operand."""
+    cache = q4rdna.KVCache(4, 16, 2, 64, device="cpu")
+    batch = q4rdna.KVBatch(torch.zeros((3, 2), dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match=r"k is \[rows, heads, 64\]"):
+        q4rdna.kv_append(cache, batch, torch.zeros((3, 3, 64)), torch.zeros((3, 2, 64)))
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        q4rdna.kv_attention(cache, batch, torch.zeros((3, 2, 64), dtype=torch.int8))

@@ -448,6 +448,23 @@ def test_attention_is_deterministic(cuda):
             assert torch.equal(q4rdna.kv_attention(cache, batch, q), first)
 
 
+def test_workspace_is_checked(cuda):
+    import ctypes
+
+    cache, _, table = make(cuda, 1210, [5000], 2, 128, 32, KV_INT8)
+    batch = KVBatch(table.to(cuda), i32([5000], cuda))
+    q = torch.randn((1, 8, 128), device=cuda)
+    a = q4rdna.KVAttentionArgs(0, 1, 8, q.data_ptr(), q.data_ptr(), 1024, 1024, 0.0, 0)
+    batch._rec.desc.max_length = 5024
+    L, ref_a, b, c = q4rdna.lib, ctypes.byref(a), ctypes.byref(batch._rec.desc), ctypes.byref(cache._rec.desc)
+    n = L.q4rdna_kv_attention_workspace_bytes(c, b, ref_a)
+    assert n > 0
+    ws = torch.empty(n + 16, dtype=torch.uint8, device=cuda)
+    assert L.q4rdna_kv_attention(c, b, ref_a, None, 0, None) == 4
+    assert L.q4rdna_kv_attention(c, b, ref_a, ws.data_ptr(), n - 1, None) == 4
+    assert L.q4rdna_kv_attention(c, b, ref_a, ws.data_ptr() + 8, n, None) == 3
+
+
 @pytest.mark.parametrize("tokens", [1, 5])
 def test_decoder_attention_block(cuda, tokens):
     """The block as a decoder runs it: RMSNorm + q/k/v products (one plan), append
