@@ -6,6 +6,7 @@
 #include <cmath>
 #include <map>
 #include <mutex>
+#include <set>
 
 #include "q4rdna_kv.h"
 #include "q4rdna_kv_append.cuh"
@@ -119,6 +120,45 @@ q4rdna_status check_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_batc
     A.scale = scale * 1.44269504088896340736f;
     A.window = args->window;
     return Q4RDNA_OK;
+}
+
+struct AppendVariant {
+    void (*kernel)(AppendArgs);
+    int smem;  // the ring; kTurnPart takes 16 rows more
+};
+template <int D, int TYPE, int FMT>
+AppendVariant append_variant(int turn) {
+    constexpr int ring = Ring<D, TYPE>::BYTES;
+    if (turn == kTurnHalves) return {kv_append_kernel<D, TYPE, FMT, kTurnHalves>, ring};
+    if (turn == kTurnPairs) return {kv_append_kernel<D, TYPE, FMT, kTurnPairs>, ring};
+    return {kv_append_kernel<D, TYPE, FMT, kTurnPart>, ring + 16 * (D + 1) * (int)sizeof(float)};
+}
+template <int D, int TYPE>
+AppendVariant append_variant(int format, int turn) {
+    return format == Q4RDNA_KV_INT8 ? append_variant<D, TYPE, Q4RDNA_KV_INT8>(turn)
+                                    : append_variant<D, TYPE, Q4RDNA_KV_E4M3>(turn);
+}
+template <int D>
+AppendVariant append_variant(int type, int format, int turn) {
+    if (type == Q4RDNA_F32) return append_variant<D, Q4RDNA_F32>(format, turn);
+    if (type == Q4RDNA_F16) return append_variant<D, Q4RDNA_F16>(format, turn);
+    return append_variant<D, Q4RDNA_BF16>(format, turn);
+}
+
+// Raises a kernel's shared-memory limit, once per device
+bool raise_smem(const void *kernel, int bytes) {
+    static std::mutex mu;
+    static std::set<std::pair<int, const void *>> done;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    std::lock_guard<std::mutex> lock(mu);
+    if (done.count({dev, kernel})) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    done.insert({dev, kernel});
+    return true;
 }
 
 // ---- the attention's launches
@@ -245,12 +285,20 @@ q4rdna_status q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_bat
     A.k = args->k; A.v = args->v; A.q = args->q; A.q_out = args->q_out;
     A.ks = args->k_stride; A.vs = args->v_stride; A.qs = args->q_stride; A.qos = args->q_out_stride;
     A.inv_freq = args->inv_freq; A.q_norm = args->q_norm; A.k_norm = args->k_norm; A.positions = args->positions;
-    A.type = args->type; A.heads = args->heads; A.rot = rot; A.neox = args->rope == Q4RDNA_ROPE_NEOX;
+    A.heads = args->heads; A.rot = rot;
     A.eps = args->norm_eps;
     const int units = batch->q_start == nullptr ? batch->sequences : args->tokens / kBlock + 2 * batch->sequences;
-    const dim3 grid((unsigned)units, (unsigned)std::min(cache->kv_heads, 65535));
-    return launch(D == 64 ? kv_append_kernel<64> : D == 128 ? kv_append_kernel<128> : kv_append_kernel<256>, grid,
-                  kAppendThreads, 0, (cudaStream_t)stream, A);
+    // Heads of a block over several CTAs where the blocks alone would not fill the GPU (each CTA makes the
+    // block's cosines anew): about 4 CTAs per SM
+    const int slices = std::max(1, std::min(std::min(cache->kv_heads, 65535), (4 * 148 + units - 1) / units));
+    const int turn = rot == 0 || (args->rope == Q4RDNA_ROPE_NEOX && rot == D) ? kTurnHalves
+                     : args->rope == Q4RDNA_ROPE_NORM                         ? kTurnPairs
+                                                                              : kTurnPart;
+    const int f = cache->format;
+    const AppendVariant v = D == 64 ? append_variant<64>(args->type, f, turn)
+                                    : D == 128 ? append_variant<128>(args->type, f, turn) : append_variant<256>(args->type, f, turn);
+    if (!raise_smem((const void *)v.kernel, v.smem)) return Q4RDNA_ERR_DEVICE;
+    return launch(v.kernel, dim3((unsigned)units, (unsigned)slices), D, v.smem, (cudaStream_t)stream, A);
 }
 
 q4rdna_status q4rdna_kv_dequant(const q4rdna_kv_cache *cache, const int32_t *page_list, int count, int type, void *k,

@@ -79,13 +79,6 @@ __device__ __forceinline__ uint8_t *tile_of(const Cache &c, const Batch &b, int 
 
 __device__ __forceinline__ float code_top(int format) { return format == Q4RDNA_KV_INT8 ? 127.0f : 448.0f; }
 
-// x (already divided by the scale) to a code: clamped, to nearest even
-__device__ __forceinline__ uint32_t to_code(float x, int format) {
-    const float top = code_top(format);
-    x = fminf(fmaxf(x, -top), top);
-    if (format == Q4RDNA_KV_INT8) return (uint32_t)__float2int_rn(x) & 0xffu;
-    return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
-}
 __device__ __forceinline__ float from_code(uint32_t code, int format) {
     if (format == Q4RDNA_KV_INT8) return (float)(int8_t)code;
     return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3)));
@@ -170,20 +163,14 @@ __device__ __forceinline__ void load_codes(const uint8_t *p, int format, float (
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = from_code((uint32_t)(w >> (8 * i)) & 0xffu, format);
 }
-// x / (sc + low) to codes: the product with inv ~ 1 / sc, corrected by its remainder,
-// so that a quotient half-way between two codes is met exactly
-template <int N>
-__device__ __forceinline__ void store_codes(uint8_t *p, int format, const float (&x)[N], float sc, float low, float inv) {
-    uint64_t w = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float y = x[i] * inv;
-        const float r = fmaf(-y, low, fmaf(-y, sc, x[i]));
-        w |= (uint64_t)to_code(fmaf(r, inv, y), format) << (8 * i);
-    }
-    if constexpr (N == 2) *reinterpret_cast<uint16_t *>(p) = (uint16_t)w;
-    else if constexpr (N == 4) *reinterpret_cast<uint32_t *>(p) = (uint32_t)w;
-    else *reinterpret_cast<uint64_t *>(p) = w;
+// ------------------------------------------------------------ asynchronous copies
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
 }  // namespace q4kv
