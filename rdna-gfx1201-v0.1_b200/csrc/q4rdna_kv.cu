@@ -1,5 +1,5 @@
 // Key/value cache operators for sm_100a, host side: argument checks and
-// launches of q4rdna_kv_append.cuh and q4rdna_kv_attention.cuh.
+// launches of q4rdna_kv_append.cuh, q4rdna_kv_attention.cuh and q4rdna_kv_tile.cuh.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -11,6 +11,7 @@
 #include "q4rdna_kv.h"
 #include "q4rdna_kv_append.cuh"
 #include "q4rdna_kv_attention.cuh"
+#include "q4rdna_kv_tile.cuh"
 
 namespace q4 {
 extern std::atomic<uint64_t> g_launches;  // q4rdna_gemv.cu: kernels launched by the library
@@ -69,8 +70,8 @@ bool known_type(int t) { return t == Q4RDNA_F32 || t == Q4RDNA_F16 || t == Q4RDN
 // One launch as a programmatic dependent of the stream's last kernel: it may be
 // set up while that one ends, and every kernel here waits for it
 // (griddepcontrol.wait) before its first access.
-template <class Args>
-q4rdna_status launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args &args) {
+template <class... Args>
+q4rdna_status launch(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args &...args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
@@ -81,7 +82,7 @@ q4rdna_status launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, 
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, args) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
         cudaGetLastError();
         return Q4RDNA_ERR_CUDA;
     }
@@ -166,13 +167,14 @@ bool raise_smem(const void *kernel, int bytes) {
 using AttnKernel = void (*)(AttnArgs);
 
 struct Variant {
-    AttnKernel split, join;
+    AttnKernel kernel;
     size_t smem;
+    int threads, nc, shift;  // columns of a task, log2 of the tokens of a piece
 };
 
 template <int D, int FMT, int NT, int TERMS>
 Variant variant() {
-    return {kv_attention_kernel<D, FMT, NT, TERMS>, kv_join_kernel<D, 8 * NT>, sizeof(AttnSmem<D, NT>)};
+    return {kv_attention_kernel<D, FMT, NT, TERMS>, sizeof(AttnSmem<D, NT>), kAttnThreads, 8 * NT, 4};
 }
 template <int D, int FMT>
 Variant variant(int nt, int terms) {
@@ -183,28 +185,34 @@ template <int D>
 Variant variant(int format, int nt, int terms) {
     return format == Q4RDNA_KV_INT8 ? variant<D, Q4RDNA_KV_INT8>(nt, terms) : variant<D, Q4RDNA_KV_E4M3>(nt, terms);
 }
+template <int D>
+Variant tile_variant(int format) {
+    return {format == Q4RDNA_KV_INT8 ? kv_tile_kernel<D, Q4RDNA_KV_INT8> : kv_tile_kernel<D, Q4RDNA_KV_E4M3>,
+            sizeof(TileSmem<D>), kTileThreads, kTileCols, kTileShift};
+}
 
+// One of the attention's kernels with its part of the workspace
 struct AttnLaunch {
-    AttnKernel split, join;
-    int nc;            // columns of a task
-    unsigned grid;     // CTAs, one share each
-    size_t smem, workspace;
+    Variant v;
+    unsigned grid;  // CTAs, one share each
+    int few, many;  // columns of the sequences that it takes
+    int min_share;
+    size_t workspace;
 };
 
-// CTAs of the split kernel that the current device holds at once (and its
-// shared-memory limit raised); 0 on an error
+// CTAs of the kernel that the current device holds at once (its shared-memory limit raised); 0 on an error
 int resident_ctas(const Variant &v) {
     static std::mutex mu;
     static std::map<std::pair<int, AttnKernel>, int> known;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
     std::lock_guard<std::mutex> lock(mu);
-    int &n = known[{dev, v.split}];
+    int &n = known[{dev, v.kernel}];
     if (n == 0) {
         int sms = 0, occ = 0;
         if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-            cudaFuncSetAttribute(v.split, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem) != cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, v.split, kAttnThreads, v.smem) != cudaSuccess) {
+            cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, v.kernel, v.threads, v.smem) != cudaSuccess) {
             cudaGetLastError();
             return 0;
         }
@@ -213,24 +221,46 @@ int resident_ctas(const Variant &v) {
     return n;
 }
 
-q4rdna_status plan_attention(AttnArgs &A, int D, AttnLaunch &L) {
-    // one column tile where a token's heads fit it and each sequence has one token, else two
-    const int nt = A.b.q_start == nullptr && A.group <= 8 ? 1 : 2;
-    const int terms = A.type == Q4RDNA_F32 ? 2 : 1;
-    const Variant v = D == 64 ? variant<64>(A.c.format, nt, terms)
-                              : D == 128 ? variant<128>(A.c.format, nt, terms) : variant<256>(A.c.format, nt, terms);
-    const int ctas = resident_ctas(v);
+q4rdna_status size_launch(const AttnArgs &A, int D, AttnLaunch &L) {
+    const int ctas = resident_ctas(L.v);
     if (ctas == 0) return Q4RDNA_ERR_DEVICE;
-    L.split = v.split;
-    L.join = v.join;
-    L.smem = v.smem;
-    L.nc = 8 * nt;
-    A.min_share = kAttnWarps;  // one block per warp
     // no more CTAs than the largest work has shares
-    const double tasks = ((double)A.b.T * A.group / L.nc + A.b.S) * A.c.hk;
-    const double work = tasks * (A.b.max_len / kBlock + 1);
-    L.grid = (unsigned)std::max(1.0, std::min((double)ctas, work / A.min_share + 1.0));
-    L.workspace = (size_t)L.grid * (2 * sizeof(int4) + 2 * sizeof(float) * part_floats(D, L.nc));
+    const double tasks = ((double)A.b.T * A.group / L.v.nc + A.b.S) * A.c.hk;
+    const double work = tasks * ((A.b.max_len >> L.v.shift) + 1);
+    L.grid = (unsigned)std::max(1.0, std::min((double)ctas, work / L.min_share + 1.0));
+    L.workspace = (size_t)L.grid * (2 * sizeof(int4) + 2 * sizeof(float) * part_floats(D, L.v.nc));
+    return Q4RDNA_OK;
+}
+
+// Columns from which on the tile kernel takes a sequence
+constexpr int kTileFrom = 48;
+
+// The launches of a call: sequences of few columns, sequences of many, or both
+q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &n) {
+    n = 0;
+    const long long most = A.b.q_start == nullptr ? A.group : (long long)A.b.T * A.group;  // columns of a sequence
+    const bool tiles = D <= 128 && A.type != Q4RDNA_F32 && most >= kTileFrom;
+    if (!tiles || (A.b.S > 1 && A.b.q_start != nullptr)) {
+        // one column tile where a token's heads fit it and each sequence has one token, else two
+        const int nt = A.b.q_start == nullptr && A.group <= 8 ? 1 : 2, terms = A.type == Q4RDNA_F32 ? 2 : 1;
+        AttnLaunch &l = L[n++];
+        l.v = D == 64 ? variant<64>(A.c.format, nt, terms)
+                      : D == 128 ? variant<128>(A.c.format, nt, terms) : variant<256>(A.c.format, nt, terms);
+        l.few = 0;
+        l.many = tiles ? kTileFrom : INT_MAX;
+        l.min_share = kAttnWarps;  // one block per warp
+    }
+    if (tiles) {
+        AttnLaunch &l = L[n++];
+        l.v = D == 64 ? tile_variant<64>(A.c.format) : tile_variant<128>(A.c.format);
+        l.few = n == 2 ? kTileFrom : 0;
+        l.many = INT_MAX;
+        l.min_share = 2;
+    }
+    for (int i = 0; i < n; ++i) {
+        const q4rdna_status st = size_launch(A, D, L[i]);
+        if (st != Q4RDNA_OK) return st;
+    }
     return Q4RDNA_OK;
 }
 
@@ -324,9 +354,13 @@ size_t q4rdna_kv_attention_workspace_bytes(const q4rdna_kv_cache *cache, const q
                                            const q4rdna_kv_attention_args *args) {
     using namespace q4kv;
     AttnArgs A{};
-    AttnLaunch L;
+    AttnLaunch L[2];
+    int n = 0;
     if (check_attention(cache, batch, args, A) != Q4RDNA_OK || args->tokens == 0 || batch->sequences == 0) return 0;
-    return plan_attention(A, cache->head_dim, L) == Q4RDNA_OK ? L.workspace : 0;
+    if (plan_attention(A, cache->head_dim, L, n) != Q4RDNA_OK) return 0;
+    size_t bytes = 0;
+    for (int i = 0; i < n; ++i) bytes += L[i].workspace;
+    return bytes;
 }
 
 q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
@@ -334,18 +368,34 @@ q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_
                                   q4rdna_stream_t stream) {
     using namespace q4kv;
     AttnArgs A{};
-    AttnLaunch L;
+    AttnLaunch L[2];
+    int n = 0;
     q4rdna_status st = check_attention(cache, batch, args, A);
     if (st != Q4RDNA_OK) return st;
     if (args->tokens == 0 || batch->sequences == 0) return Q4RDNA_OK;
-    if ((st = plan_attention(A, cache->head_dim, L)) != Q4RDNA_OK) return st;
-    if (workspace == nullptr || workspace_bytes < L.workspace) return Q4RDNA_ERR_WORKSPACE;
+    const int D = cache->head_dim;
+    if ((st = plan_attention(A, D, L, n)) != Q4RDNA_OK) return st;
+    size_t bytes = 0;
+    for (int i = 0; i < n; ++i) bytes += L[i].workspace;
+    if (workspace == nullptr || workspace_bytes < bytes) return Q4RDNA_ERR_WORKSPACE;
     if (!aligned(workspace)) return Q4RDNA_ERR_ALIGNMENT;
-    A.rec = reinterpret_cast<int4 *>(workspace);
-    A.part = reinterpret_cast<float *>(A.rec + 2 * L.grid);
     const cudaStream_t cs = (cudaStream_t)stream;
-    if ((st = launch(L.split, dim3(L.grid), kAttnThreads, L.smem, cs, A)) != Q4RDNA_OK) return st;
-    return launch(L.join, dim3(L.grid), 32 * L.nc, 0, cs, A);
+    const auto join = D == 64 ? kv_join_kernel<64> : D == 128 ? kv_join_kernel<128> : kv_join_kernel<256>;
+    uint8_t *at = reinterpret_cast<uint8_t *>(workspace);
+    for (int i = 0; i < n; ++i) {
+        const AttnLaunch &l = L[i];
+        A.few = l.few;
+        A.many = l.many;
+        A.min_share = l.min_share;
+        A.rec = reinterpret_cast<int4 *>(at);
+        A.part = reinterpret_cast<float *>(A.rec + 2 * l.grid);
+        at += l.workspace;
+        if ((st = launch(l.v.kernel, dim3(l.grid), l.v.threads, l.v.smem, cs, A)) != Q4RDNA_OK) return st;
+        if ((st = launch(join, dim3(l.grid, (unsigned)((l.v.nc + kJoinWarps - 1) / kJoinWarps)), 32 * kJoinWarps, 0, cs, A,
+                         l.v.nc)) != Q4RDNA_OK)
+            return st;
+    }
+    return Q4RDNA_OK;
 }
 
 }  // extern "C"

@@ -1,17 +1,7 @@
-// Attention over the 8-bit cache, few columns per sequence (q4rdna_kv_attention).
+// Attention over the 8-bit cache, few columns per sequence (q4rdna_kv_attention): a task
+// (q4rdna_kv_split.cuh) is NC = 8 NT columns, its pieces the 16-token blocks.
+// HBM-bound: every block is read once per task, 2 D + 1/2 bytes per token and head.
 //
-// A column is one query row (token, head); the columns of a kv head are all the
-// query heads of its group for all the sequence's new tokens.  A task is (sequence,
-// kv head, group of NC = 8 NT columns); its work is the 16-token blocks that any of
-// its columns sees.  HBM-bound: every block is read once per task, 2 D + 1/2 bytes
-// per token and head.
-//
-//   * Split: all tasks' blocks in a row are cut into equal shares, one per CTA
-//     (as many CTAs as the GPU holds at once), so a batch of uneven lengths and a
-//     single long sequence fill the GPU alike.  A task that lies in several shares
-//     leaves one partial result (maximum, sum, NC x D sums) per share, and
-//     kv_join_kernel, launched behind as a programmatic dependent, adds them in
-//     share order: no atomics, no order that changes a result.
 //   * A CTA's 8 warps take its blocks in turn and meet in shared memory at the end
 //     of a task's blocks.
 //   * Scores on the tensor cores: S^T = K q^T as mma.m16n8k16 with f16 operands and
@@ -32,55 +22,14 @@
 //     dims D/8 g .. of tokens 4 c .. 4 c + 3 (lane = 4 g + c).
 #pragma once
 
-#include "q4rdna_kv.cuh"
+#include "q4rdna_kv_split.cuh"
 
 namespace q4kv {
 
-struct AttnArgs {
-    Cache c;
-    Batch b;
-    const void *q;
-    void *out;
-    int64_t qs, os;
-    int type, heads, group;
-    float scale;    // of q . k, times log2(e)
-    int window;     // 0: none
-    int min_share;  // blocks per CTA at least
-    float *part;    // partial results: two slots per CTA
-    int4 *rec;      // per CTA: the task that begins in its share and goes on
-};
-
 constexpr int kAttnWarps = 8;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr float kBoost = 7.0f;   // p carries 2^7
-constexpr float kStep = 8.0f;    // m moves when a score outgrows it by more
-
-// Floats of one partial result
-__host__ __device__ constexpr int part_floats(int D, int NC) { return NC * (D + 2); }
-
-// The columns col0 .. col0 + NC - 1 of a sequence: blocks [lo, hi) that any of them sees
-struct Span {
-    int lo, hi;
-};
-__device__ __forceinline__ Span span_of(const Seq &q, int col0, int nc, int group, int window) {
-    const int i0 = col0 / group, i1 = min(q.n - 1, (col0 + nc - 1) / group);
-    const int p0 = q.L - q.n + i0, p1 = q.L - q.n + i1;
-    Span s;
-    s.hi = p1 < 0 ? 0 : (p1 >> 4) + 1;
-    s.lo = window > 0 ? min(max(0, p0 - window + 1) >> 4, s.hi) : 0;
-    return s;
-}
-// Work of a task: one block at least, so that every task lies in a share and its rows are written
-__device__ __forceinline__ int work_of(const Span &s) { return max(1, s.hi - s.lo); }
-
-// Work of one kv head of a sequence
-__device__ __forceinline__ long long head_work(const Seq &q, int nc, int group, int window) {
-    const int cols = q.n * group;
-    if (nc >= cols) return cols == 0 ? 0 : work_of(span_of(q, 0, nc, group, window));
-    long long w = 0;
-    for (int c = 0; c < cols; c += nc) w += work_of(span_of(q, c, nc, group, window));
-    return w;
-}
+constexpr float kBoost = 7.0f;  // p carries 2^7
+constexpr float kStep = 8.0f;   // m moves when a score outgrows it by more
 
 // ------------------------------------------------------------ fragments
 
@@ -97,22 +46,6 @@ __device__ __forceinline__ uint2 ld_stream2(const uint8_t *p) {
     return v;
 }
 
-__device__ __forceinline__ uint32_t sub_1152(uint32_t x) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));
-    return r;
-}
-
-// Two codes to two f16 numbers, exact.  int8: `w` holds code ^ 0x80; byte b under the
-// exponent byte 0x64 is 1024 + b, less 1152 the code.  e4m3: the byte's exponent and
-// mantissa moved to f16's place are 2^-8 times the number (subnormals too).
-// (a, b): codes number LO and LO + 1 of one word
-template <int FMT, int LO>
-__device__ __forceinline__ uint32_t pair_of(uint32_t w) {
-    if constexpr (FMT == Q4RDNA_KV_INT8) return sub_1152(__byte_perm(w, 0x64646464u, LO == 0 ? 0x4140 : 0x4342));
-    const uint32_t p = __byte_perm(w, 0u, LO == 0 ? 0x1404 : 0x3424);
-    return ((p >> 1) & 0x3f803f80u) | (p & 0x80008000u);
-}
 // (a, b): code number I of the words a and b (two tokens, one dim)
 template <int FMT>
 __device__ __forceinline__ void pairs_of(uint32_t a, uint32_t b, uint32_t (&r)[4]) {
@@ -144,16 +77,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_half(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // ------------------------------------------------------------ the kernel
 
 template <int D, int NT>
@@ -165,63 +88,8 @@ struct AttnSmem {
     float qscale[NC];
     float o[kAttnWarps][NC][OROW];
     float m[kAttnWarps][NC], l[kAttnWarps][NC];
-    long long sum[kAttnWarps];
-    long long rest;  // offset of the share's begin in sequence `seq`
-    long long share;
-    int seq;
+    ShareSmem<kAttnWarps> share;
 };
-
-// Where the CTA's share begins: sequence, offset in its work, and the share's length (0: nothing)
-template <class Smem>
-__device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, Smem &sm) {
-    const Batch &B = A.b;
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto work = [&](int s) -> long long {
-        return s < B.S ? head_work(load_seq(B, s), nc, A.group, A.window) * A.c.hk : 0;
-    };
-    const long long first = work(threadIdx.x);  // of a chunk of 256 sequences; most batches are one
-    long long total = 0;
-    for (int base = 0; base < B.S; base += kAttnThreads) {
-        long long x = base == 0 ? first : work(base + threadIdx.x);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        if (lane == 0) sm.sum[w] = x;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kAttnWarps; ++i) total += sm.sum[i];
-        __syncthreads();
-    }
-    const long long share = max((long long)A.min_share, (total + gridDim.x - 1) / gridDim.x);
-    const long long begin = share * blockIdx.x;
-    if (begin >= total) return 0;
-    if (threadIdx.x == 0) sm.share = share;
-    long long before = 0;
-    for (int base = 0; base < B.S && before <= begin; base += kAttnThreads) {
-        const long long mine = base == 0 ? first : work(base + threadIdx.x);
-        long long x = mine;  // inclusive prefix
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        if (lane == 31) sm.sum[w] = x;
-        __syncthreads();
-        long long all = 0;
-#pragma unroll
-        for (int i = 0; i < kAttnWarps; ++i) {
-            if (i < w) x += sm.sum[i];
-            all += sm.sum[i];
-        }
-        const long long at = begin - before - (x - mine);
-        if (at >= 0 && at < mine) {
-            sm.seq = base + threadIdx.x;
-            sm.rest = at;
-        }
-        before += all;
-        __syncthreads();
-    }
-    return min(share, total - begin);
-}
 
 template <int D, int FMT, int NT, int TERMS>
 __global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1)
@@ -237,387 +105,321 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    long long left = find_share(A, NC, sm);
+    const long long left = find_share<kAttnWarps>(A, NC, 4, sm.share);
     if (left == 0) {
         if (threadIdx.x == 0) A.rec[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
         return;
     }
-    const long long share = sm.share;
-    long long rest = sm.rest;
-    int s = sm.seq;
     bool open = false;  // the share ends inside a task that began in it
     const int t0 = 4 * (g >> 1) + (g & 1);  // K rows g and g + 8 of the fragments: tokens t0 and t0 + 2
-    while (left > 0) {
-        const Seq sq = load_seq(B, s);
-        const int cols = sq.n * A.group;
-        const long long hw = head_work(sq, NC, A.group, A.window);
-        if (hw == 0) { ++s; continue; }
-        int h = (int)(rest / hw);
-        rest -= h * hw;
-        for (; h < A.c.hk && left > 0; ++h) {
-            for (int col0 = 0; col0 < cols && left > 0; col0 += NC) {
-                const Span sp = span_of(sq, col0, NC, A.group, A.window);
-                const int all = work_of(sp);
-                if (rest >= all) { rest -= all; continue; }
-                const int b0 = sp.lo + (int)rest;
-                const int cnt = (int)min((long long)(all - (int)rest), left);
-                const int b1 = min(b0 + cnt, sp.hi);
-                const bool begins = rest == 0, ends = (int)rest + cnt == all;
-                rest = 0;
-                left -= cnt;
-                const int first = sq.L - sq.n;  // token of the sequence's first row
+    Walk W(A, NC, 4, left, sm.share.rest, sm.share.share, sm.share.seq);
+    while (W.next()) {
+        const Seq &sq = W.q;
+        const int s = W.s, cols = W.cols, h = W.h, col0 = W.col0, b0 = W.begin, b1 = W.end;
+        const int first = sq.L - sq.n;  // token of the sequence's first row
 
-                // ---- q of the columns, scaled to f16
-                __syncthreads();  // the last task's join has read shared memory
-                for (int j = w; j < NC; j += kAttnWarps) {
-                    const int col = col0 + j;
-                    float x[D / 32];
-                    uint32_t mx = 0;
-                    if (col < cols) {
-                        const int i = col / A.group;
-                        load_row<D / 32>(A.q, (size_t)(sq.a + i) * A.qs +
-                                                  ((size_t)h * A.group + (col - i * A.group)) * D + lane * (D / 32),
-                                         A.type, x);
-                    }
+        // ---- q of the columns, scaled to f16
+        __syncthreads();  // the last task's join has read shared memory
+        for (int j = w; j < NC; j += kAttnWarps) {
+            const int col = col0 + j;
+            float x[D / 32];
+            uint32_t mx = 0;
+            if (col < cols) {
+                const int i = col / A.group;
+                load_row<D / 32>(A.q, (size_t)(sq.a + i) * A.qs +
+                                          ((size_t)h * A.group + (col - i * A.group)) * D + lane * (D / 32),
+                                 A.type, x);
+            }
 #pragma unroll
-                    for (int t = 0; t < D / 32; ++t) {
-                        if (col >= cols) x[t] = 0.0f;
-                        mx = max(mx, __float_as_uint(x[t]) & 0x7fffffffu);
-                    }
-                    mx = __reduce_max_sync(0xffffffffu, mx);
-                    // the largest |q| to [2^13, 2^14); exponents beyond +-100 stay
-                    int e = 140 - (int)(mx >> 23);
-                    e = mx == 0 || mx >= 0x7f800000u ? 0 : max(-100, min(100, e));
-                    const float f = __int_as_float((127 + e) << 23);
+            for (int t = 0; t < D / 32; ++t) {
+                if (col >= cols) x[t] = 0.0f;
+                mx = max(mx, __float_as_uint(x[t]) & 0x7fffffffu);
+            }
+            mx = __reduce_max_sync(0xffffffffu, mx);
+            // the largest |q| to [2^13, 2^14); exponents beyond +-100 stay
+            int e = 140 - (int)(mx >> 23);
+            e = mx == 0 || mx >= 0x7f800000u ? 0 : max(-100, min(100, e));
+            const float f = __int_as_float((127 + e) << 23);
 #pragma unroll
-                    for (int t = 0; t < D / 32; t += 2) {
-                        const float a = x[t] * f, b = x[t + 1] * f;
-                        const uint32_t hi = pack_half(a, b);
-                        *reinterpret_cast<uint32_t *>(&sm.q[0][j][lane * (D / 32) + t]) = hi;
-                        if constexpr (TERMS == 2) {
-                            const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-                            *reinterpret_cast<uint32_t *>(&sm.q[1][j][lane * (D / 32) + t]) = pack_half(a - r.x, b - r.y);
-                        }
-                    }
-                    if (lane == 0)
-                        sm.qscale[j] = A.scale * __int_as_float((127 - e) << 23) * (FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f);
+            for (int t = 0; t < D / 32; t += 2) {
+                const float a = x[t] * f, b = x[t + 1] * f;
+                const uint32_t hi = pack_half(a, b);
+                *reinterpret_cast<uint32_t *>(&sm.q[0][j][lane * (D / 32) + t]) = hi;
+                if constexpr (TERMS == 2) {
+                    const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                    *reinterpret_cast<uint32_t *>(&sm.q[1][j][lane * (D / 32) + t]) = pack_half(a - r.x, b - r.y);
                 }
-                __syncthreads();
+            }
+            if (lane == 0)
+                sm.qscale[j] = A.scale * __int_as_float((127 - e) << 23) * (FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f);
+        }
+        __syncthreads();
 
-                // ---- this warp's blocks
-                float o[NT][MT][4], m[NT][2], l[NT][2], cs[NT][2];
-                int plo[NT][2], phi[NT][2];  // tokens that the lane's columns see
+        // ---- this warp's blocks
+        float o[NT][MT][4], m[NT][2], l[NT][2], cs[NT][2];
+        int plo[NT][2], phi[NT][2];  // tokens that the lane's columns see
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) o[n][i][z] = 0.0f;
+                for (int z = 0; z < 4; ++z) o[n][i][z] = 0.0f;
 #pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        m[n][z] = -INFINITY;
-                        l[n][z] = 0.0f;
-                        const int col = col0 + 8 * n + 2 * c + z;
-                        cs[n][z] = sm.qscale[8 * n + 2 * c + z];
-                        phi[n][z] = col < cols ? first + col / A.group : -1;
-                        plo[n][z] = A.window > 0 ? phi[n][z] - A.window + 1 : 0;
+            for (int z = 0; z < 2; ++z) {
+                m[n][z] = -INFINITY;
+                l[n][z] = 0.0f;
+                const int col = col0 + 8 * n + 2 * c + z;
+                cs[n][z] = sm.qscale[8 * n + 2 * c + z];
+                phi[n][z] = col < cols ? first + col / A.group : -1;
+                plo[n][z] = A.window > 0 ? phi[n][z] - A.window + 1 : 0;
+            }
+        }
+        // blocks that every column sees whole need no mask (padded columns are all zero and never read)
+        const int last = first + min(sq.n - 1, (col0 + NC - 1) / A.group);
+        const int full_hi = (first + col0 / A.group + 1) >> 4;  // first block that is not whole below
+        const int full_lo = A.window > 0 ? (max(0, last - A.window + 1) + 15) >> 4 : 0;
+
+        uint4 kr[2][KW];
+        uint32_t vr[4][VB / 4];
+        float2 sc = make_float2(0.0f, 0.0f);
+        auto load_k = [&](const uint8_t *tile) {
+#pragma unroll
+            for (int i = 0; i < KW; ++i) {
+                kr[0][i] = ld_stream(tile + kHeader + t0 * D + 16 * c + 64 * i);
+                kr[1][i] = ld_stream(tile + kHeader + (t0 + 2) * D + 16 * c + 64 * i);
+            }
+        };
+        auto load_v = [&](const uint8_t *tile) {
+            const uint8_t *p = tile + kHeader + (kBlock + 4 * c) * D + VB * g;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if constexpr (VB == 8) {
+                    const uint2 x = ld_stream2(p + t * D);
+                    vr[t][0] = x.x; vr[t][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VB / 16; ++i) {
+                        const uint4 x = ld_stream(p + t * D + 16 * i);
+                        vr[t][4 * i] = x.x; vr[t][4 * i + 1] = x.y; vr[t][4 * i + 2] = x.z; vr[t][4 * i + 3] = x.w;
                     }
                 }
-                // blocks that every column sees whole need no mask (padded columns are all zero and never read)
-                const int last = first + min(sq.n - 1, (col0 + NC - 1) / A.group);
-                const int full_hi = (first + col0 / A.group + 1) >> 4;  // first block that is not whole below
-                const int full_lo = A.window > 0 ? (max(0, last - A.window + 1) + 15) >> 4 : 0;
+            }
+        };
+        // the next block of this warp whose page lies in the cache
+        auto next_tile = [&](int &b) -> const uint8_t * {
+            for (; b < b1; b += kAttnWarps) {
+                const uint8_t *t = tile_of(A.c, B, s, h, b);
+                if (t != nullptr) return t;
+            }
+            return nullptr;
+        };
+        int b = b0 + w;
+        const uint8_t *tile = next_tile(b);
+        if (tile != nullptr) {
+            load_k(tile);
+            load_v(tile);
+            sc = __ldg(reinterpret_cast<const float2 *>(tile));
+        }
+        while (tile != nullptr) {
+            const int cur = b;
+            b += kAttnWarps;
+            const uint8_t *next = next_tile(b);
 
-                uint4 kr[2][KW];
-                uint32_t vr[4][VB / 4];
-                float2 sc = make_float2(0.0f, 0.0f);
-                auto load_k = [&](const uint8_t *tile) {
+            // scores
+            float sa[NT][TERMS][4];
 #pragma unroll
-                    for (int i = 0; i < KW; ++i) {
-                        kr[0][i] = ld_stream(tile + kHeader + t0 * D + 16 * c + 64 * i);
-                        kr[1][i] = ld_stream(tile + kHeader + (t0 + 2) * D + 16 * c + 64 * i);
-                    }
-                };
-                auto load_v = [&](const uint8_t *tile) {
-                    const uint8_t *p = tile + kHeader + (kBlock + 4 * c) * D + VB * g;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        if constexpr (VB == 8) {
-                            const uint2 x = ld_stream2(p + t * D);
-                            vr[t][0] = x.x; vr[t][1] = x.y;
-                        } else {
+                for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-                            for (int i = 0; i < VB / 16; ++i) {
-                                const uint4 x = ld_stream(p + t * D + 16 * i);
-                                vr[t][4 * i] = x.x; vr[t][4 * i + 1] = x.y; vr[t][4 * i + 2] = x.z; vr[t][4 * i + 3] = x.w;
-                            }
-                        }
+                    for (int z = 0; z < 4; ++z) sa[n][t][z] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KW; ++i) {
+                const uint32_t r0[4] = {kr[0][i].x, kr[0][i].y, kr[0][i].z, kr[0][i].w};
+                const uint32_t r1[4] = {kr[1][i].x, kr[1][i].y, kr[1][i].z, kr[1][i].w};
+                uint32_t qf[NT][TERMS][8];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t) {
+                        const uint4 *p = reinterpret_cast<const uint4 *>(&sm.q[t][8 * n + g][64 * i + 16 * c]);
+                        const uint4 x = p[0], y = p[1];
+                        qf[n][t][0] = x.x; qf[n][t][1] = x.y; qf[n][t][2] = x.z; qf[n][t][3] = x.w;
+                        qf[n][t][4] = y.x; qf[n][t][5] = y.y; qf[n][t][6] = y.z; qf[n][t][7] = y.w;
                     }
-                };
-                // the next block of this warp whose page lies in the cache
-                auto next_tile = [&](int &b) -> const uint8_t * {
-                    for (; b < b1; b += kAttnWarps) {
-                        const uint8_t *t = tile_of(A.c, B, s, h, b);
-                        if (t != nullptr) return t;
-                    }
-                    return nullptr;
-                };
-                int b = b0 + w;
-                const uint8_t *tile = next_tile(b);
-                if (tile != nullptr) {
-                    load_k(tile);
-                    load_v(tile);
-                    sc = __ldg(reinterpret_cast<const float2 *>(tile));
-                }
-                while (tile != nullptr) {
-                    const int cur = b;
-                    b += kAttnWarps;
-                    const uint8_t *next = next_tile(b);
-
-                    // scores
-                    float sa[NT][TERMS][4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t x0 = FMT == Q4RDNA_KV_INT8 ? r0[u] ^ 0x80808080u : r0[u];
+                    const uint32_t x1 = FMT == Q4RDNA_KV_INT8 ? r1[u] ^ 0x80808080u : r1[u];
+                    const uint32_t a0 = pair_of<FMT, 0>(x0), a2 = pair_of<FMT, 2>(x0);
+                    const uint32_t a1 = pair_of<FMT, 0>(x1), a3 = pair_of<FMT, 2>(x1);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-                            for (int z = 0; z < 4; ++z) sa[n][t][z] = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < KW; ++i) {
-                        const uint32_t r0[4] = {kr[0][i].x, kr[0][i].y, kr[0][i].z, kr[0][i].w};
-                        const uint32_t r1[4] = {kr[1][i].x, kr[1][i].y, kr[1][i].z, kr[1][i].w};
-                        uint32_t qf[NT][TERMS][8];
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int t = 0; t < TERMS; ++t) {
-                                const uint4 *p = reinterpret_cast<const uint4 *>(&sm.q[t][8 * n + g][64 * i + 16 * c]);
-                                const uint4 x = p[0], y = p[1];
-                                qf[n][t][0] = x.x; qf[n][t][1] = x.y; qf[n][t][2] = x.z; qf[n][t][3] = x.w;
-                                qf[n][t][4] = y.x; qf[n][t][5] = y.y; qf[n][t][6] = y.z; qf[n][t][7] = y.w;
-                            }
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const uint32_t x0 = FMT == Q4RDNA_KV_INT8 ? r0[u] ^ 0x80808080u : r0[u];
-                            const uint32_t x1 = FMT == Q4RDNA_KV_INT8 ? r1[u] ^ 0x80808080u : r1[u];
-                            const uint32_t a0 = pair_of<FMT, 0>(x0), a2 = pair_of<FMT, 2>(x0);
-                            const uint32_t a1 = pair_of<FMT, 0>(x1), a3 = pair_of<FMT, 2>(x1);
-#pragma unroll
-                            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                for (int t = 0; t < TERMS; ++t)
-                                    mma_f16(sa[n][t], a0, a1, a2, a3, qf[n][t][2 * u], qf[n][t][2 * u + 1]);
-                        }
-                    }
-                    const float2 scale = sc;
-                    if (next != nullptr) {
-                        load_k(next);
-                        sc = __ldg(reinterpret_cast<const float2 *>(next));
-                    }
-
-                    // softmax weights; lane: tokens t0, t0 + 2 of columns 2 c, 2 c + 1
-                    const bool whole = cur >= full_lo && cur < full_hi;
-                    uint32_t pf[NT][TERMS][2];
-                    float sv[NT][2];
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float x[4];
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            x[z] = sa[n][0][z];
-                            if constexpr (TERMS == 2) x[z] += sa[n][1][z];
-                            x[z] *= scale.x * cs[n][z & 1];
-                        }
-                        sv[n][0] = sv[n][1] = scale.y * (FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f);
-                        if (!whole) {
-#pragma unroll
-                            for (int z = 0; z < 4; ++z) {
-                                const int tok = cur * kBlock + t0 + (z & 2);
-                                if (tok > phi[n][z & 1] || tok < plo[n][z & 1]) x[z] = -INFINITY;
-                            }
-#pragma unroll
-                            for (int z = 0; z < 2; ++z)  // a column that sees nothing here takes nothing from the tile's scale
-                                if (cur * kBlock > phi[n][z] || cur * kBlock + kBlock - 1 < plo[n][z]) sv[n][z] = 0.0f;
-                        }
-                        float f[2];
-                        bool moved = false;
-#pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            float y = fmaxf(x[z], x[z + 2]);
-                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
-                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
-                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
-                            f[z] = 1.0f;
-                            if (y > m[n][z] + kStep) {  // also the first score: m = -inf
-                                f[z] = ex2(m[n][z] - y);
-                                m[n][z] = y;
-                                moved = true;
-                            }
-                        }
-                        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                                for (int z = 0; z < 4; ++z) o[n][i][z] *= f[z & 1];
-                            l[n][0] *= f[0];
-                            l[n][1] *= f[1];
-                        }
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const float ref = m[n][z & 1];
-                            x[z] = ex2(x[z] - (ref == -INFINITY ? 0.0f : ref) + kBoost);
-                            l[n][z & 1] += x[z];
-                        }
-#pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            const uint32_t hi = pack_half(x[2 * z], x[2 * z + 1]);
-                            pf[n][0][z] = transpose8(hi);
-                            if constexpr (TERMS == 2) {
-                                const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-                                pf[n][1][z] = transpose8(pack_half(x[2 * z] - r.x, x[2 * z + 1] - r.y));
-                            }
-                        }
-                    }
-
-                    // values
-#pragma unroll
-                    for (int u = 0; u < VB / 4; ++u) {
-                        uint32_t lo[4], hi[4];
-                        if constexpr (FMT == Q4RDNA_KV_INT8) {
-                            pairs_of<FMT>(vr[0][u] ^ 0x80808080u, vr[1][u] ^ 0x80808080u, lo);
-                            pairs_of<FMT>(vr[2][u] ^ 0x80808080u, vr[3][u] ^ 0x80808080u, hi);
-                        } else {
-                            pairs_of<FMT>(vr[0][u], vr[1][u], lo);
-                            pairs_of<FMT>(vr[2][u], vr[3][u], hi);
-                        }
-#pragma unroll
-                        for (int v = 0; v < 2; ++v)
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                                for (int t = 0; t < TERMS; ++t)
-                                    mma_f16(acc, lo[2 * v], lo[2 * v + 1], hi[2 * v], hi[2 * v + 1], pf[n][t][0], pf[n][t][1]);
-#pragma unroll
-                                for (int z = 0; z < 4; ++z)
-                                    o[n][2 * u + v][z] = fmaf(sv[n][z & 1], acc[z], o[n][2 * u + v][z]);
-                            }
-                    }
-                    if (next != nullptr) load_v(next);
-                    tile = next;
-                }
-
-                // ---- the warps meet
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        const int j = 8 * n + 2 * c + z;
-                        float x = l[n][z];
-                        x += __shfl_xor_sync(0xffffffffu, x, 4);
-                        x += __shfl_xor_sync(0xffffffffu, x, 8);
-                        x += __shfl_xor_sync(0xffffffffu, x, 16);
-                        if (g == 0) {
-                            sm.m[w][j] = m[n][z];
-                            sm.l[w][j] = x;
-                        }
-#pragma unroll
-                        for (int i = 0; i < MT; ++i)  // M tile i: dims VB g + 2 i (rows g) and + 1 (rows g + 8)
-                            *reinterpret_cast<float2 *>(&sm.o[w][j][VB * g + 2 * i]) =
-                                make_float2(o[n][i][z], o[n][i][z + 2]);
-                    }
-                __syncthreads();
-                const bool whole_task = begins && ends;
-                float *part = A.part + (size_t)(2 * blockIdx.x + (begins ? 1 : 0)) * part_floats(D, NC);
-                for (int e = threadIdx.x; e < NC * (D / 4); e += kAttnThreads) {
-                    const int j = e / (D / 4), d = 4 * (e % (D / 4));
-                    const int col = col0 + j;
-                    if (col >= cols) continue;
-                    float M = -INFINITY, L = 0.0f, f[kAttnWarps];
-#pragma unroll
-                    for (int i = 0; i < kAttnWarps; ++i) M = fmaxf(M, sm.m[i][j]);
-                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int i = 0; i < kAttnWarps; ++i) {
-                        // a warp that saw nothing has l = 0 and o = 0, or NaN, which goes through
-                        f[i] = sm.m[i][j] == -INFINITY ? 1.0f : ex2(sm.m[i][j] - M);
-                        L = fmaf(f[i], sm.l[i][j], L);
-                        const float4 y = *reinterpret_cast<const float4 *>(&sm.o[i][j][d]);
-                        x[0] = fmaf(f[i], y.x, x[0]);
-                        x[1] = fmaf(f[i], y.y, x[1]);
-                        x[2] = fmaf(f[i], y.z, x[2]);
-                        x[3] = fmaf(f[i], y.w, x[3]);
-                    }
-                    if (whole_task) {
-                        const float r = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) x[z] *= r;
-                        const int i = col / A.group;
-                        store_row<4>(A.out, (size_t)(sq.a + i) * A.os + ((size_t)h * A.group + (col - i * A.group)) * D + d,
-                                     A.type, x);
-                    } else {
-                        *reinterpret_cast<float4 *>(part + j * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-                        if (d == 0) {
-                            part[NC * D + j] = M;
-                            part[NC * D + NC + j] = L;
-                        }
-                    }
-                }
-                if (begins && !ends && threadIdx.x == 0) {
-                    open = true;
-                    A.rec[2 * blockIdx.x] = make_int4(1, sq.a, cols, col0);
-                    A.rec[2 * blockIdx.x + 1] = make_int4(h, (int)blockIdx.x + (int)((all - cnt + share - 1) / share), 0, 0);
+                            mma_f16(sa[n][t], a0, a1, a2, a3, qf[n][t][2 * u], qf[n][t][2 * u + 1]);
                 }
             }
-            rest = 0;
+            const float2 scale = sc;
+            if (next != nullptr) {
+                load_k(next);
+                sc = __ldg(reinterpret_cast<const float2 *>(next));
+            }
+
+            // softmax weights; lane: tokens t0, t0 + 2 of columns 2 c, 2 c + 1
+            const bool whole = cur >= full_lo && cur < full_hi;
+            uint32_t pf[NT][TERMS][2];
+            float sv[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float x[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    x[z] = sa[n][0][z];
+                    if constexpr (TERMS == 2) x[z] += sa[n][1][z];
+                    x[z] *= scale.x * cs[n][z & 1];
+                }
+                sv[n][0] = sv[n][1] = scale.y * (FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f);
+                if (!whole) {
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const int tok = cur * kBlock + t0 + (z & 2);
+                        if (tok > phi[n][z & 1] || tok < plo[n][z & 1]) x[z] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int z = 0; z < 2; ++z)  // a column that sees nothing here takes nothing from the tile's scale
+                        if (cur * kBlock > phi[n][z] || cur * kBlock + kBlock - 1 < plo[n][z]) sv[n][z] = 0.0f;
+                }
+                float f[2];
+                bool moved = false;
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    float y = fmaxf(x[z], x[z + 2]);
+                    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+                    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+                    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                    f[z] = 1.0f;
+                    if (y > m[n][z] + kStep) {  // also the first score: m = -inf
+                        f[z] = ex2(m[n][z] - y);
+                        m[n][z] = y;
+                        moved = true;
+                    }
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) o[n][i][z] *= f[z & 1];
+                    l[n][0] *= f[0];
+                    l[n][1] *= f[1];
+                }
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    const float ref = m[n][z & 1];
+                    x[z] = ex2(x[z] - (ref == -INFINITY ? 0.0f : ref) + kBoost);
+                    l[n][z & 1] += x[z];
+                }
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    const uint32_t hi = pack_half(x[2 * z], x[2 * z + 1]);
+                    pf[n][0][z] = transpose8(hi);
+                    if constexpr (TERMS == 2) {
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                        pf[n][1][z] = transpose8(pack_half(x[2 * z] - r.x, x[2 * z + 1] - r.y));
+                    }
+                }
+            }
+
+            // values
+#pragma unroll
+            for (int u = 0; u < VB / 4; ++u) {
+                uint32_t lo[4], hi[4];
+                if constexpr (FMT == Q4RDNA_KV_INT8) {
+                    pairs_of<FMT>(vr[0][u] ^ 0x80808080u, vr[1][u] ^ 0x80808080u, lo);
+                    pairs_of<FMT>(vr[2][u] ^ 0x80808080u, vr[3][u] ^ 0x80808080u, hi);
+                } else {
+                    pairs_of<FMT>(vr[0][u], vr[1][u], lo);
+                    pairs_of<FMT>(vr[2][u], vr[3][u], hi);
+                }
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int t = 0; t < TERMS; ++t)
+                            mma_f16(acc, lo[2 * v], lo[2 * v + 1], hi[2 * v], hi[2 * v + 1], pf[n][t][0], pf[n][t][1]);
+#pragma unroll
+                        for (int z = 0; z < 4; ++z)
+                            o[n][2 * u + v][z] = fmaf(sv[n][z & 1], acc[z], o[n][2 * u + v][z]);
+                    }
+            }
+            if (next != nullptr) load_v(next);
+            tile = next;
         }
-        ++s;
+
+        // ---- the warps meet
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const int j = 8 * n + 2 * c + z;
+                float x = l[n][z];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (g == 0) {
+                    sm.m[w][j] = m[n][z];
+                    sm.l[w][j] = x;
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i)  // M tile i: dims VB g + 2 i (rows g) and + 1 (rows g + 8)
+                    *reinterpret_cast<float2 *>(&sm.o[w][j][VB * g + 2 * i]) =
+                        make_float2(o[n][i][z], o[n][i][z + 2]);
+            }
+        __syncthreads();
+        const bool whole_task = W.whole();
+        float *part = W.part(D);
+        for (int e = threadIdx.x; e < NC * (D / 4); e += kAttnThreads) {
+            const int j = e / (D / 4), d = 4 * (e % (D / 4));
+            const int col = col0 + j;
+            if (col >= cols) continue;
+            float M = -INFINITY, L = 0.0f, f[kAttnWarps];
+#pragma unroll
+            for (int i = 0; i < kAttnWarps; ++i) M = fmaxf(M, sm.m[i][j]);
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kAttnWarps; ++i) {
+                // a warp that saw nothing has l = 0 and o = 0, or NaN, which goes through
+                f[i] = sm.m[i][j] == -INFINITY ? 1.0f : ex2(sm.m[i][j] - M);
+                L = fmaf(f[i], sm.l[i][j], L);
+                const float4 y = *reinterpret_cast<const float4 *>(&sm.o[i][j][d]);
+                x[0] = fmaf(f[i], y.x, x[0]);
+                x[1] = fmaf(f[i], y.y, x[1]);
+                x[2] = fmaf(f[i], y.z, x[2]);
+                x[3] = fmaf(f[i], y.w, x[3]);
+            }
+            if (whole_task) {
+                const float r = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) x[z] *= r;
+                const int i = col / A.group;
+                store_row<4>(A.out, (size_t)(sq.a + i) * A.os + ((size_t)h * A.group + (col - i * A.group)) * D + d,
+                             A.type, x);
+            } else {
+                *reinterpret_cast<float4 *>(part + j * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+                if (d == 0) {
+                    part[NC * D + j] = M;
+                    part[NC * D + NC + j] = L;
+                }
+            }
+        }
+        if (W.open()) {
+            open = true;
+            if (threadIdx.x == 0) W.note();
+        }
     }
     if (threadIdx.x == 0 && !open) A.rec[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-}
-
-// Joins the pieces of the task that began in CTA blockIdx.x's share and went on
-// in the next ones: one warp per column.
-template <int D, int NC>
-__global__ void __launch_bounds__(32 * NC) kv_join_kernel(const __grid_constant__ AttnArgs A) {
-    constexpr int EPL = D / 32;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 r0 = A.rec[2 * blockIdx.x];
-    if (r0.x == 0) return;
-    const int4 r1 = A.rec[2 * blockIdx.x + 1];
-    const int j = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int col = r0.w + j;
-    if (col >= r0.z) return;
-    // piece 0: this CTA's second slot; then the first slots of the CTAs up to the task's last
-    auto piece = [&](int i) {
-        return A.part + (size_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * part_floats(D, NC);
-    };
-    const int n = min(r1.y, (int)gridDim.x - 1) - (int)blockIdx.x + 1;
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, piece(i)[NC * D + j]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float x[EPL], L = 0.0f;
-#pragma unroll
-    for (int t = 0; t < EPL; ++t) x[t] = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const float *p = piece(i);
-        const float mi = p[NC * D + j];
-        const float f = mi == -INFINITY ? 1.0f : ex2(mi - M);
-        L = fmaf(f, p[NC * D + NC + j], L);
-        float y[EPL];
-        load_row<EPL>(p, (size_t)j * D + lane * EPL, Q4RDNA_F32, y);
-#pragma unroll
-        for (int t = 0; t < EPL; ++t) x[t] = fmaf(f, y[t], x[t]);
-    }
-    const float r = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-    for (int t = 0; t < EPL; ++t) x[t] *= r;
-    const int i = col / A.group;
-    store_row<EPL>(A.out, (size_t)(r0.y + i) * A.os + ((size_t)r1.x * A.group + (col - i * A.group)) * D + lane * EPL, A.type,
-                   x);
 }
 
 }  // namespace q4kv

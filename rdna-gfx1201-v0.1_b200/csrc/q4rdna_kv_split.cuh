@@ -1,0 +1,257 @@
+// What the attention's kernels share: arguments, the cut of all tasks' work into
+// equal shares, the decoding of two codes to f16, and the join of partial results.
+//
+// A column is one query row (token, head); the columns of a kv head are all the
+// query heads of its group for all the sequence's new tokens.  A task is (sequence,
+// kv head, group of nc columns); its work is the pieces of 2^shift tokens that any of
+// its columns sees.  All tasks' work in a row is cut into equal shares, one per CTA
+// (as many CTAs as the GPU holds at once), so a batch of uneven lengths and a single
+// long sequence fill the GPU alike.  A task that lies in several shares leaves one
+// partial result (maximum, sum, nc x D sums) per share, and kv_join_kernel, launched
+// behind as a programmatic dependent, adds them in share order: no atomics, no order
+// that changes a result.
+#pragma once
+
+#include "q4rdna_kv.cuh"
+
+namespace q4kv {
+
+struct AttnArgs {
+    Cache c;
+    Batch b;
+    const void *q;
+    void *out;
+    int64_t qs, os;
+    int type, heads, group;
+    float scale;    // of q . k, times log2(e)
+    int window;     // 0: none
+    int min_share;  // pieces per CTA at least
+    int few, many;  // only sequences of few <= columns < many
+    float *part;    // partial results: two slots per CTA
+    int4 *rec;      // per CTA: the task that begins in its share and goes on
+};
+
+// Floats of one partial result
+__host__ __device__ constexpr int part_floats(int D, int NC) { return NC * (D + 2); }
+
+// The columns col0 .. col0 + nc - 1 of a sequence: pieces [lo, hi) that any of them sees
+struct Span {
+    int lo, hi;
+};
+__device__ __forceinline__ Span span_of(const Seq &q, int col0, int nc, int group, int window, int shift) {
+    const int i0 = col0 / group, i1 = min(q.n - 1, (col0 + nc - 1) / group);
+    const int p0 = q.L - q.n + i0, p1 = q.L - q.n + i1;
+    Span s;
+    s.hi = p1 < 0 ? 0 : (p1 >> shift) + 1;
+    s.lo = window > 0 ? min(max(0, p0 - window + 1) >> shift, s.hi) : 0;
+    return s;
+}
+// Work of a task: one piece at least, so that every task lies in a share and its rows are written
+__device__ __forceinline__ int work_of(const Span &s) { return max(1, s.hi - s.lo); }
+
+// Work of one kv head of a sequence; 0 for a sequence that is not this kernel's
+__device__ __forceinline__ long long head_work(const AttnArgs &A, const Seq &q, int nc, int shift) {
+    const int cols = q.n * A.group;
+    if (cols < A.few || cols >= A.many) return 0;
+    if (nc >= cols) return cols == 0 ? 0 : work_of(span_of(q, 0, nc, A.group, A.window, shift));
+    long long w = 0;
+    for (int c = 0; c < cols; c += nc) w += work_of(span_of(q, c, nc, A.group, A.window, shift));
+    return w;
+}
+
+template <int WARPS>
+struct ShareSmem {
+    long long sum[WARPS];
+    long long rest;  // offset of the share's begin in sequence `seq`
+    long long share;
+    int seq;
+};
+
+// Where the CTA's share begins: sequence and offset in its work (in sm); returns the
+// share's length (0: nothing).  All of the CTA's threads take part.
+template <int WARPS>
+__device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int shift, ShareSmem<WARPS> &sm) {
+    constexpr int THREADS = 32 * WARPS;
+    const Batch &B = A.b;
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto work = [&](int s) -> long long { return s < B.S ? head_work(A, load_seq(B, s), nc, shift) * A.c.hk : 0; };
+    const long long first = work(threadIdx.x);  // of a chunk of THREADS sequences; most batches are one
+    long long total = 0;
+    for (int base = 0; base < B.S; base += THREADS) {
+        long long x = base == 0 ? first : work(base + threadIdx.x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (lane == 0) sm.sum[w] = x;
+        __syncthreads();
+        for (int i = 0; i < WARPS; ++i) total += sm.sum[i];
+        __syncthreads();
+    }
+    const long long share = max((long long)A.min_share, (total + gridDim.x - 1) / gridDim.x);
+    const long long begin = share * blockIdx.x;
+    if (begin >= total) return 0;
+    if (threadIdx.x == 0) sm.share = share;
+    long long before = 0;
+    for (int base = 0; base < B.S && before <= begin; base += THREADS) {
+        const long long mine = base == 0 ? first : work(base + threadIdx.x);
+        long long x = mine;  // inclusive prefix
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) sm.sum[w] = x;
+        __syncthreads();
+        long long all = 0;
+        for (int i = 0; i < WARPS; ++i) {
+            if (i < w) x += sm.sum[i];
+            all += sm.sum[i];
+        }
+        const long long at = begin - before - (x - mine);
+        if (at >= 0 && at < mine) {
+            sm.seq = base + threadIdx.x;
+            sm.rest = at;
+        }
+        before += all;
+        __syncthreads();
+    }
+    return min(share, total - begin);
+}
+
+// The tasks of a share, one after the other (the same in all threads)
+struct Walk {
+    const AttnArgs &A;
+    int nc, shift;
+    long long left, rest, share;
+    int s;
+    Seq q{};
+    int cols = 0, h = 0, col0 = 0;
+    // the piece of the current task that is this share's
+    Span span{};
+    int begin = 0, end = 0, all = 0, cnt = 0;
+    bool begins = false, ends = false;
+
+    __device__ __forceinline__ Walk(const AttnArgs &a, int nc_, int shift_, long long left_, long long rest_, long long share_,
+                                    int seq)
+        : A(a), nc(nc_), shift(shift_), left(left_), rest(rest_), share(share_), s(seq - 1), h(a.c.hk) {}
+
+    __device__ __forceinline__ bool next() {
+        if (left <= 0) return false;
+        col0 += nc;
+        while (true) {
+            if (col0 >= cols) {  // the next head, or the next sequence with work
+                col0 = 0;
+                if (++h >= A.c.hk) {
+                    long long hw;
+                    do {
+                        if (++s >= A.b.S) return false;
+                        q = load_seq(A.b, s);
+                        hw = head_work(A, q, nc, shift);
+                    } while (hw == 0);
+                    cols = q.n * A.group;
+                    h = (int)(rest / hw);
+                    rest -= h * hw;
+                }
+            }
+            span = span_of(q, col0, nc, A.group, A.window, shift);
+            all = work_of(span);
+            if (rest < all) break;
+            rest -= all;
+            col0 += nc;
+        }
+        begin = span.lo + (int)rest;
+        cnt = (int)min((long long)(all - (int)rest), left);
+        end = min(begin + cnt, span.hi);
+        begins = rest == 0;
+        ends = (int)rest + cnt == all;
+        rest = 0;
+        left -= cnt;
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return begins && ends; }
+    // this piece's partial result
+    __device__ __forceinline__ float *part(int D) const {
+        return A.part + (size_t)(2 * blockIdx.x + (begins ? 1 : 0)) * part_floats(D, nc);
+    }
+    // the share ends inside a task that began in it: what the join needs
+    __device__ __forceinline__ void note() const {
+        A.rec[2 * blockIdx.x] = make_int4(1, q.a, cols, col0);
+        A.rec[2 * blockIdx.x + 1] = make_int4(h, (int)blockIdx.x + (int)((all - cnt + share - 1) / share), 0, 0);
+    }
+    __device__ __forceinline__ bool open() const { return begins && !ends; }
+};
+
+// ------------------------------------------------------------ codes to f16
+
+__device__ __forceinline__ uint32_t sub_1152(uint32_t x) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));
+    return r;
+}
+
+// Two codes to two f16 numbers, exact.  int8: `w` holds code ^ 0x80; byte b under the
+// exponent byte 0x64 is 1024 + b, less 1152 the code.  e4m3: the byte's exponent and
+// mantissa moved to f16's place are 2^-8 times the number (subnormals too).
+// (a, b): codes number LO and LO + 1 of one word
+template <int FMT, int LO>
+__device__ __forceinline__ uint32_t pair_of(uint32_t w) {
+    if constexpr (FMT == Q4RDNA_KV_INT8) return sub_1152(__byte_perm(w, 0x64646464u, LO == 0 ? 0x4140 : 0x4342));
+    const uint32_t p = __byte_perm(w, 0u, LO == 0 ? 0x1404 : 0x3424);
+    return ((p >> 1) & 0x3f803f80u) | (p & 0x80008000u);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Joins the pieces of the task that began in CTA blockIdx.x's share and went on
+// in the next ones: one warp per column, blockIdx.y the eighth columns.
+constexpr int kJoinWarps = 8;
+template <int D>
+__global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_constant__ AttnArgs A, int nc) {
+    constexpr int EPL = D / 32;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 r0 = A.rec[2 * blockIdx.x];
+    if (r0.x == 0) return;
+    const int4 r1 = A.rec[2 * blockIdx.x + 1];
+    const int j = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int col = r0.w + j;
+    if (col >= r0.z) return;
+    // piece 0: this CTA's second slot; then the first slots of the CTAs up to the task's last
+    auto piece = [&](int i) {
+        return A.part + (size_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * part_floats(D, nc);
+    };
+    const int n = min(r1.y, (int)gridDim.x - 1) - (int)blockIdx.x + 1;
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, piece(i)[nc * D + j]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float x[EPL], L = 0.0f;
+#pragma unroll
+    for (int t = 0; t < EPL; ++t) x[t] = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float *p = piece(i);
+        const float mi = p[nc * D + j];
+        const float f = mi == -INFINITY ? 1.0f : ex2(mi - M);
+        L = fmaf(f, p[nc * D + nc + j], L);
+        float y[EPL];
+        load_row<EPL>(p, (size_t)j * D + lane * EPL, Q4RDNA_F32, y);
+#pragma unroll
+        for (int t = 0; t < EPL; ++t) x[t] = fmaf(f, y[t], x[t]);
+    }
+    const float r = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int t = 0; t < EPL; ++t) x[t] *= r;
+    const int i = col / A.group;
+    store_row<EPL>(A.out, (size_t)(r0.y + i) * A.os + ((size_t)r1.x * A.group + (col - i * A.group)) * D + lane * EPL, A.type,
+                   x);
+}
+
+}  // namespace q4kv

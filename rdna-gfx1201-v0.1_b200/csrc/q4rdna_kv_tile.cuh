@@ -1,0 +1,560 @@
+// Attention over the 8-bit cache, many columns per sequence: prompts and pieces of
+// prompts (q4rdna_kv_attention), on the 5th-generation tensor cores.
+//
+// A task (q4rdna_kv_split.cuh) is 256 columns as two tiles of 128 rows; its pieces are
+// steps of 128 tokens.  Bound by the tensor cores and the exponentials alike: a step
+// takes 2 x (128 x 128 x D) x 2 products (2048 cycles at D = 128) and 2 x 128 x 128
+// exponentials (2048 cycles at 16 a cycle).
+//   * One persistent CTA per SM, 16 warps (128 registers; a 17th would leave 96):
+//       warps 0-3, 4-7   softmax of tile 0 and tile 1, one row per thread;
+//       warps 8-14       read the cache's 8-bit tiles, write K and V as f16;
+//       warp 15          one thread issues the products.
+//   * S = Q K^T: tcgen05.mma kind::f16, M = 128, N = 128, f32 in tensor memory; Q and
+//     the codes of K (exact in f16) in shared memory, K-major with 128-byte swizzle.
+//   * O += P V: P in f16 as the A operand in tensor memory, over the first half of S's
+//     columns; V as it lies (dims contiguous: the MN-major B operand), 128-byte
+//     swizzle.  O stays in tensor memory over a task.
+//   * While one tile's softmax runs, the other tile's products do.
+//   * Scales: a block's key scale multiplies its 16 columns of S, the logarithm of its
+//     value scale joins the exponent, p = 2^(s + log2 sv - R); the sum of the weights
+//     themselves takes each block's sum times 1 / sv.  R, per row, moves only when an
+//     exponent outgrows it by 8 (the row's O is then rescaled by its own thread), and p
+//     carries 2^7: f16 holds weights from 2^15 to 2^-24.
+//   * Tensor memory (512 columns): S0 S1 O0 O1, 128 each.
+// Every wait is bounded (about a second, %globaltimer): on expiry the role sets bit 4
+// of the fault word and takes no more waits, copies or products; the issuing thread
+// still waits (bounded) for its products before the tensor memory is freed.
+#pragma once
+
+#include <climits>
+
+#include "q4rdna_kv_split.cuh"
+
+namespace q4kv {
+
+constexpr int kTileWarps = 16, kTileLoadWarps = 7, kTileMmaWarp = 15;
+constexpr int kTileThreads = 32 * kTileWarps;
+constexpr int kTileRows = 128, kTileTokens = 128, kTileCols = 256, kTileShift = 7;
+constexpr int kTileLoaders = 32 * kTileLoadWarps;
+constexpr unsigned kFaultTile = 16u;
+constexpr uint64_t kTileWaitNs = 1000000000ull;
+
+template <int D>
+struct TileSmem {
+    static constexpr int PANEL = kTileTokens * 128;       // 128 rows of 64 f16, swizzled
+    static constexpr int STAGE = PANEL * (D / 64);        // a K or V stage, or a tile's Q
+    uint8_t q[2][STAGE];
+    uint8_t k[2][STAGE];
+    uint8_t v[2][STAGE];
+    float4 scale[4][8];  // per block of a step: key scale, log2 and inverse of the value scale
+    float qscale[2][kTileRows];
+    uint64_t bar[24];
+    ShareSmem<kTileWarps> share;
+    uint32_t tmem;
+};
+
+// ------------------------------------------------------------ PTX
+
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity) {
+    uint64_t t0, t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    for (uint32_t n = 1;; ++n) {
+        if (bar_try(bar, parity)) return true;
+        if ((n & 63u) == 0) {
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+            if (t - t0 > kTileWaitNs) return false;
+        }
+    }
+}
+// Waits for the phase of the given parity; `ok` false: not any more
+__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, bool &ok) {
+    if (ok && !bar_try(bar, parity)) {
+        ok = bar_wait_slow(bar, parity);
+        if (!ok) atomicOr(&g_kv_fault, kFaultTile);
+    }
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Shared-memory operand, 128-byte swizzle: stride 1024 between groups of 8 rows;
+// `lead` between panels of 64 elements (MN-major only)
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+        "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(addr)
+        : "memory");
+}
+
+// Byte of element (row, chunk of 8) of a swizzled operand of 64-element panels
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
+    return (uint32_t)((chunk >> 3) * (kTileTokens * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+// ------------------------------------------------------------ softmax of one row
+
+struct RowState {
+    float R, l;        // reference of the exponents, sum of the weights
+    float scale;       // of the row's scores
+    int lo, hi;        // tokens that the row sees: [lo, hi]
+};
+
+// One step of one row: S to P.  MASK: some row of the warp does not see all of it.
+template <bool MASK>
+__device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, uint32_t s_at, uint32_t o_at, int od, int tok0,
+                                             bool first) {
+    // the largest exponent
+    float t = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tmem_load32(s_at + 32 * c, v);
+        tmem_wait_load();
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const float4 f = scale[2 * c + b];
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float x = __uint_as_float(v[16 * b + i]);
+                if constexpr (MASK) {
+                    const int tok = tok0 + 32 * c + 16 * b + i;
+                    m = fmaxf(m, tok < r.lo || tok > r.hi ? -INFINITY : x);
+                } else {
+                    m = fmaxf(m, x);
+                }
+            }
+            const float a = f.x * r.scale;
+            // a block without a visible token has m = -inf, which a scale of 0 would turn into NaN
+            if (MASK) t = fmaxf(t, m == -INFINITY ? -INFINITY : fmaf(m, a, f.y));
+            else t = fmaxf(t, fmaf(m, a, f.y));
+        }
+    }
+    float f = 1.0f;
+    const bool moved = t > r.R + 8.0f;  // also the first: R = -inf
+    if (moved) {
+        f = ex2(r.R - t);
+        r.R = t;
+        r.l *= f;
+    }
+    if (__any_sync(0xffffffffu, moved) && !first) {
+        // the products of the step before have ended (they come before this S), the next ones wait for this P
+        for (int c = 0; c < od; c += 32) {
+            uint32_t v[32];
+            tmem_load32(o_at + c, v);
+            tmem_wait_load();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+            tmem_store32(o_at + c, v);
+        }
+    }
+    const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t v[32], p[16];
+        tmem_load32(s_at + 32 * c, v);
+        tmem_wait_load();
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const float4 g = scale[2 * c + b];
+            const float a = g.x * r.scale, d = g.y - ref;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                float e[2];
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    float x = fmaf(__uint_as_float(v[16 * b + i + z]), a, d);
+                    if constexpr (MASK) {
+                        const int tok = tok0 + 32 * c + 16 * b + i + z;
+                        if (tok < r.lo || tok > r.hi) x = -INFINITY;
+                    }
+                    e[z] = ex2(x);
+                }
+                sum += e[0] + e[1];
+                p[8 * b + i / 2] = pack_half(e[0], e[1]);
+            }
+            // a block without a visible token takes nothing from its scale, be it NaN
+            if (!MASK || sum != 0.0f) r.l = fmaf(sum, g.z, r.l);
+        }
+        // P's column 16 c lies on S's columns that are done
+        tmem_store16(s_at + 16 * c, p);
+    }
+    tmem_wait_store();
+}
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_constant__ AttnArgs A) {
+    using Smem = TileSmem<D>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
+    const Batch &B = A.b;
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t bar0 = smem_u32(sm.bar);
+    // mbarriers: K and V stage full / empty, scales (ring of 4), and per tile Q written, S
+    // computed, P written, O complete
+    auto k_full = [&](int i) { return bar0 + 8u * i; };
+    auto k_empty = [&](int i) { return bar0 + 8u * (2 + i); };
+    auto v_full = [&](int i) { return bar0 + 8u * (4 + i); };
+    auto v_empty = [&](int i) { return bar0 + 8u * (6 + i); };
+    auto sc_full = [&](int i) { return bar0 + 8u * (8 + i); };
+    auto q_full = [&](int x) { return bar0 + 8u * (12 + x); };
+    auto s_full = [&](int x) { return bar0 + 8u * (14 + x); };
+    auto p_full = [&](int x) { return bar0 + 8u * (16 + x); };
+    auto o_full = [&](int x) { return bar0 + 8u * (18 + x); };
+    const uint32_t drained = bar0 + 8u * 20;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (w == kTileMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            bar_init(k_full(i), kTileLoadWarps);
+            bar_init(v_full(i), kTileLoadWarps);
+            bar_init(k_empty(i), 1);
+            bar_init(v_empty(i), 1);
+            bar_init(q_full(i), 4);
+            bar_init(s_full(i), 1);
+            bar_init(p_full(i), 4);
+            bar_init(o_full(i), 1);
+        }
+        for (int i = 0; i < 4; ++i) bar_init(sc_full(i), 1);
+        bar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sm.tmem;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const long long left = find_share<kTileWarps>(A, kTileCols, kTileShift, sm.share);
+    bool ok = true, open = false;
+    if (left > 0) {
+        Walk W(A, kTileCols, kTileShift, left, sm.share.rest, sm.share.share, sm.share.seq);
+        uint32_t it = 0;   // steps so far: stage it % 2
+        uint32_t st[2] = {0, 0}, tt[2] = {0, 0};  // steps of either tile, and tasks with steps
+        while (W.next()) {
+            const Seq &sq = W.q;
+            const int steps = max(0, W.end - W.begin);
+            const int rows = W.cols - W.col0;            // columns of the task, 256 at most count
+            const int tiles = rows > kTileRows ? 2 : 1;
+            const int first = sq.L - sq.n;               // token of the sequence's first row
+            if (w < 8) {
+                // ------------------------------------------------ softmax
+                const int x = w >> 2;
+                const int rt = threadIdx.x & 127;  // row of the tile = TMEM lane
+                if (x < tiles) {
+                    if (steps > 0) {
+                        // Q: one row per warp and turn, scaled by a power of two to f16
+#pragma unroll 2
+                        for (int i = 0; i < 32; ++i) {
+                            const int r = 32 * (w & 3) + i, col = W.col0 + kTileRows * x + r;
+                            constexpr int N = D / 32;
+                            float y[N];
+                            uint32_t mx = 0;
+                            if (col < W.cols) {
+                                const int t = col / A.group;
+                                load_row<N>(A.q, (size_t)(sq.a + t) * A.qs + ((size_t)W.h * A.group + (col - t * A.group)) * D + lane * N,
+                                            A.type, y);
+                            }
+#pragma unroll
+                            for (int z = 0; z < N; ++z) {
+                                if (col >= W.cols) y[z] = 0.0f;
+                                mx = max(mx, __float_as_uint(y[z]) & 0x7fffffffu);
+                            }
+                            mx = __reduce_max_sync(0xffffffffu, mx);
+                            int e = 140 - (int)(mx >> 23);  // the largest |q| to [2^13, 2^14)
+                            e = mx == 0 || mx >= 0x7f800000u ? 0 : max(-100, min(100, e));
+                            const float f = __int_as_float((127 + e) << 23);
+                            uint32_t p[N / 2];
+#pragma unroll
+                            for (int z = 0; z < N / 2; ++z) p[z] = pack_half(y[2 * z] * f, y[2 * z + 1] * f);
+                            uint8_t *to = sm.q[x] + swizzled(r, lane * N / 8) + (lane * N % 8) * 2;
+                            if constexpr (N == 2) *reinterpret_cast<uint32_t *>(to) = p[0];
+                            else *reinterpret_cast<uint2 *>(to) = make_uint2(p[0], p[1]);
+                            if (lane == 0) sm.qscale[x][r] = A.scale * __int_as_float((127 - e) << 23);
+                        }
+                        fence_async();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(q_full(x));
+                    }
+                    RowState r;
+                    const int col = W.col0 + kTileRows * x + rt;
+                    const bool there = col < W.cols;
+                    r.R = -INFINITY;
+                    r.l = 0.0f;
+                    r.scale = steps > 0 ? sm.qscale[x][rt] : 0.0f;  // written by this warp
+                    r.hi = there ? first + col / A.group : INT_MAX;  // (a padded row is computed and never read)
+                    r.lo = there && A.window > 0 ? max(0, r.hi - A.window + 1) : 0;
+                    // tokens that all rows of the warp see
+                    const int all_lo = __reduce_max_sync(0xffffffffu, r.lo), all_hi = __reduce_min_sync(0xffffffffu, r.hi);
+                    const uint32_t lanes = (uint32_t)(32 * (w & 3)) << 16;
+                    const uint32_t s_at = tmem + lanes + 128 * x, o_at = tmem + lanes + 256 + 128 * x;
+                    for (int j = 0; j < steps; ++j) {
+                        const uint32_t n = it + j;
+                        bar_wait(s_full(x), st[x] & 1, ok);
+                        bar_wait(sc_full(n & 3), (n >> 2) & 1, ok);  // at most one phase ahead once S is there
+                        ++st[x];
+                        fence_after();
+                        const int tok0 = (W.begin + j) * kTileTokens;
+                        if (tok0 >= all_lo && tok0 + kTileTokens - 1 <= all_hi)
+                            softmax_step<false>(r, sm.scale[n & 3], s_at, o_at, D, tok0, j == 0);
+                        else
+                            softmax_step<true>(r, sm.scale[n & 3], s_at, o_at, D, tok0, j == 0);
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(p_full(x));
+                    }
+                    // the result
+                    if (steps > 0) bar_wait(o_full(x), tt[x] & 1, ok);
+                    if (steps > 0) ++tt[x];
+                    fence_after();
+                    const bool whole = W.whole();
+                    const float inv = r.l == 0.0f ? 0.0f : 1.0f / r.l;
+                    float *part = W.part(D);
+                    const int j = kTileRows * x + rt;
+                    const int tok = there ? col / A.group : 0;
+                    const size_t at = (size_t)(sq.a + tok) * A.os + ((size_t)W.h * A.group + (there ? col - tok * A.group : 0)) * D;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t v[32];
+                        if (steps > 0) {
+                            tmem_load32(o_at + c, v);
+                            tmem_wait_load();
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = 0;
+                        }
+                        if (there) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                float y[8];
+#pragma unroll
+                                for (int z = 0; z < 8; ++z) y[z] = __uint_as_float(v[i + z]) * (whole ? inv : 1.0f);
+                                if (whole) store_row<8>(A.out, at + c + i, A.type, y);
+                                else store_row<8>(part, (size_t)j * D + c + i, Q4RDNA_F32, y);
+                            }
+                        }
+                    }
+                    if (there && !whole) {
+                        part[kTileCols * D + j] = r.R;
+                        part[kTileCols * D + kTileCols + j] = r.l;
+                    }
+                    fence_before();
+                }
+            } else if (w < kTileMmaWarp) {
+                // ------------------------------------------------ loading
+                const int u = threadIdx.x - 256;
+                constexpr int PIECES = D / 16;                             // 16 codes each, of a token
+                constexpr int STEP = kTileLoaders / PIECES;                // tokens from piece to piece of a thread
+                constexpr int N = (kTileTokens + STEP - 1) / STEP;         // pieces of a thread, K or V of a step
+                const int ch = u % PIECES, tk = u / PIECES;
+                // 16-token blocks that a column of the task sees
+                const Span sp = span_of(sq, W.col0, kTileCols, A.group, A.window, 4);
+                auto tile_at = [&](int blk) -> const uint8_t * {  // null: nothing to read, zeros
+                    return blk >= sp.lo && blk < sp.hi ? tile_of(A.c, B, W.s, W.h, blk) : nullptr;
+                };
+                uint4 kr[N], vr[N];
+                const uint8_t *at[N];
+                auto find = [&](int step) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        at[i] = tk + i * STEP < kTileTokens ? tile_at(step * 8 + (tk + i * STEP) / 16) : nullptr;
+                    }
+                };
+                auto load = [&](uint4(&r)[N], int z) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const int t = (tk + i * STEP) & 15;
+                        r[i] = at[i] == nullptr ? make_uint4(0, 0, 0, 0)
+                                                : *reinterpret_cast<const uint4 *>(at[i] + kHeader + (z * kBlock + t) * D + 16 * ch);
+                    }
+                };
+                auto put = [&](uint8_t *stage, const uint4(&r)[N]) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const int t = tk + i * STEP;
+                        if (t >= kTileTokens) break;
+                        const uint32_t wd[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+                        uint32_t h[8];
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            const uint32_t y = FMT == Q4RDNA_KV_INT8 ? wd[z] ^ 0x80808080u : wd[z];
+                            h[2 * z] = pair_of<FMT, 0>(y);
+                            h[2 * z + 1] = pair_of<FMT, 2>(y);
+                        }
+                        // the two halves in an order that keeps a phase's lanes in different banks
+                        const bool odd = (ch >> 2) & 1;
+                        const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
+                        *reinterpret_cast<uint4 *>(stage + swizzled(t, 2 * ch + (odd ? 1 : 0))) = odd ? b : a;
+                        *reinterpret_cast<uint4 *>(stage + swizzled(t, 2 * ch + (odd ? 0 : 1))) = odd ? a : b;
+                    }
+                    fence_async();
+                    __syncwarp();
+                };
+                if (steps > 0) {
+                    find(W.begin);
+                    load(kr, 0);
+                    load(vr, 1);
+                }
+                for (int j = 0; j < steps; ++j) {
+                    const uint32_t n = it + j;
+                    const int stage = n & 1;
+                    const uint32_t parity = ((n >> 1) & 1) ^ 1;
+                    float2 hd = make_float2(0.0f, 0.0f);
+                    if (w == 8 && lane < 8) {
+                        const uint8_t *t = tile_at((W.begin + j) * 8 + lane);
+                        if (t != nullptr) hd = *reinterpret_cast<const float2 *>(t);
+                    }
+                    bar_wait(k_empty(stage), parity, ok);
+                    put(sm.k[stage], kr);
+                    if (lane == 0) bar_arrive(k_full(stage));
+                    if (w == 8) {
+                        if (lane < 8) {
+                            constexpr float M = FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f;  // e4m3 numbers come as 2^-8 of theirs
+                            const float sv = hd.y <= kTinyScale ? kTinyScale : hd.y * M;  // NaN stays
+                            sm.scale[n & 3][lane] = make_float4(hd.x * M, log2f(sv), 1.0f / sv, 0.0f);
+                        }
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(sc_full(n & 3));
+                    }
+                    if (j + 1 < steps) {
+                        find(W.begin + j + 1);
+                        load(kr, 0);
+                    }
+                    bar_wait(v_empty(stage), parity, ok);
+                    put(sm.v[stage], vr);
+                    if (lane == 0) bar_arrive(v_full(stage));
+                    if (j + 1 < steps) load(vr, 1);
+                }
+            } else if (lane == 0) {
+                // ------------------------------------------------ products
+                // f16 operands, f32 sums, M = 128; S: both K-major, N = 128; O: B MN-major, N = D
+                constexpr uint32_t S_DESC = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | (8u << 24);
+                constexpr uint32_t O_DESC = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+                auto scores = [&](int x, int stage) {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint32_t off = (i >> 2) * Smem::PANEL + (i & 3) * 32;
+                        mma_ss(tmem + 128 * x, operand(smem_u32(sm.q[x]) + off, 16), operand(smem_u32(sm.k[stage]) + off, 16),
+                               S_DESC, i > 0);
+                    }
+                    commit(s_full(x));
+                };
+                if (steps > 0) {
+                    for (int x = 0; x < tiles; ++x) bar_wait(q_full(x), tt[x] & 1, ok);
+                    bar_wait(k_full(it & 1), (it >> 1) & 1, ok);
+                    fence_after();
+                    if (ok) {
+                        for (int x = 0; x < tiles; ++x) scores(x, it & 1);
+                        commit(k_empty(it & 1));
+                    }
+                }
+                for (int j = 0; j < steps; ++j) {
+                    const uint32_t n = it + j;
+                    if (j + 1 < steps) bar_wait(k_full((n + 1) & 1), ((n + 1) >> 1) & 1, ok);
+                    bar_wait(v_full(n & 1), (n >> 1) & 1, ok);
+                    for (int x = 0; x < tiles; ++x) {
+                        bar_wait(p_full(x), st[x] & 1, ok);
+                        ++st[x];
+                        fence_after();
+                        if (!ok) continue;
+#pragma unroll
+                        for (int i = 0; i < kTileTokens / 16; ++i)
+                            mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * i,
+                                   operand(smem_u32(sm.v[n & 1]) + i * 2048, Smem::PANEL), O_DESC, j > 0 || i > 0);
+                        if (j + 1 == steps) commit(o_full(x));
+                        else scores(x, (n + 1) & 1);
+                    }
+                    if (ok) {
+                        commit(v_empty(n & 1));
+                        if (j + 1 < steps) commit(k_empty((n + 1) & 1));
+                    }
+                }
+                for (int x = 0; x < tiles && steps > 0; ++x) ++tt[x];
+            }
+            it += steps;
+            if (W.open()) {
+                open = true;
+                if (threadIdx.x == 0) W.note();
+            }
+        }
+    }
+    if (threadIdx.x == 0 && !open) A.rec[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (w == kTileMmaWarp && lane == 0) {  // no product may still run when the tensor memory goes
+        bool last = true;
+        commit(drained);
+        bar_wait(drained, 0, last);
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (w == kTileMmaWarp) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace q4kv
