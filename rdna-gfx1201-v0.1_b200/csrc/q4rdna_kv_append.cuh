@@ -53,34 +53,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// Two f32 numbers in one register pair: one instruction for both
-typedef unsigned long long F2;
-__device__ __forceinline__ F2 pack2(float a, float b) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 both(F2 x) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-    return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 // Which elements of a row a lane holds: 8 of either half, as 16-byte pieces that
 // lie side by side over the lanes (16-bit types: 8 elements at 8 l; f32: 4 at 4 l
 // of either quarter; 32 bytes per lane would fetch every 32-byte sector twice)

@@ -150,44 +150,62 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
     return (uint32_t)((chunk >> 3) * (kTileTokens * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
-// ------------------------------------------------------------ softmax of one row
+// ------------------------------------------------------------ softmax
 
 struct RowState {
-    float R, l;        // reference of the exponents, sum of the weights
-    float scale;       // of the row's scores
-    int lo, hi;        // tokens that the row sees: [lo, hi]
+    float R, l;    // reference of the exponents, sum of the weights
+    float scale;   // of the row's scores
+    int lo, hi;    // tokens that the row sees: [lo, hi]
+};
+
+// Where a softmax warp works and what it waits for
+struct RowPlace {
+    uint32_t s_at, o_at;                // tensor memory of the warp's rows
+    uint32_t s_full, p_full, sc_full;   // mbarriers (sc_full: the first of four)
+    uint32_t steps, it, parity;         // of the task; steps before it, of the CTA and (parity of S) of the tile
+    int tok0, all_lo, all_hi;           // first token of the task; tokens that all rows of the warp see
 };
 
 // One step of one row: S to P.  MASK: some row of the warp does not see all of it.
-template <bool MASK>
-__device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, uint32_t s_at, uint32_t o_at, int od, int tok0,
+// S is read twice, 32 columns ahead of the arithmetic, rather than held (128 registers).
+template <int D, bool MASK>
+__device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, uint32_t s_at, uint32_t o_at, int tok0,
                                              bool first) {
-    // the largest exponent
+    uint32_t v0[32], v1[32];
+    // columns 32 c .. of S: the largest exponent
     float t = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tmem_load32(s_at + 32 * c, v);
-        tmem_wait_load();
+    auto largest = [&](const uint32_t(&v)[32], int c) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const float4 f = scale[2 * c + b];
-            float m = -INFINITY;
+            float m[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = __uint_as_float(v[16 * b + i]);
-                if constexpr (MASK) {
-                    const int tok = tok0 + 32 * c + 16 * b + i;
-                    m = fmaxf(m, tok < r.lo || tok > r.hi ? -INFINITY : x);
-                } else {
-                    m = fmaxf(m, x);
+            for (int i = 0; i < 16; i += 2) {
+                float x[2];
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    x[z] = __uint_as_float(v[16 * b + i + z]);
+                    if constexpr (MASK) {
+                        const int tok = tok0 + 32 * c + 16 * b + i + z;
+                        if (tok < r.lo || tok > r.hi) x[z] = -INFINITY;
+                    }
                 }
+                m[i / 2 & 1] = fmaxf(fmaxf(m[i / 2 & 1], x[0]), x[1]);
             }
-            const float a = f.x * r.scale;
-            // a block without a visible token has m = -inf, which a scale of 0 would turn into NaN
-            if (MASK) t = fmaxf(t, m == -INFINITY ? -INFINITY : fmaf(m, a, f.y));
-            else t = fmaxf(t, fmaf(m, a, f.y));
+            const float mx = fmaxf(m[0], m[1]), y = fmaf(mx, f.x * r.scale, f.y);
+            // a block without a visible token has mx = -inf, which a scale of 0 would turn into NaN
+            t = fmaxf(t, MASK && mx == -INFINITY ? -INFINITY : y);
         }
+    };
+    tmem_load32(s_at, v0);
+#pragma unroll 1
+    for (int c = 0; c < 4; c += 2) {
+        tmem_wait_load();
+        tmem_load32(s_at + 32 * (c + 1), v1);
+        largest(v0, c);
+        tmem_wait_load();
+        tmem_load32(s_at + 32 * ((c + 2) & 3), v0);  // at the end the next pass's first
+        largest(v1, c + 1);
     }
     float f = 1.0f;
     const bool moved = t > r.R + 8.0f;  // also the first: R = -inf
@@ -198,48 +216,172 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
     }
     if (__any_sync(0xffffffffu, moved) && !first) {
         // the products of the step before have ended (they come before this S), the next ones wait for this P
-        for (int c = 0; c < od; c += 32) {
-            uint32_t v[32];
-            tmem_load32(o_at + c, v);
+        tmem_wait_load();
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            tmem_load32(o_at + c, v1);
             tmem_wait_load();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-            tmem_store32(o_at + c, v);
+            for (int i = 0; i < 32; ++i) v1[i] = __float_as_uint(__uint_as_float(v1[i]) * f);
+            tmem_store32(o_at + c, v1);
         }
     }
     const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t v[32], p[16];
-        tmem_load32(s_at + 32 * c, v);
-        tmem_wait_load();
+    auto weights = [&](const uint32_t(&v)[32], int c) {
+        uint32_t p[16];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const float4 g = scale[2 * c + b];
             const float a = g.x * r.scale, d = g.y - ref;
-            float sum = 0.0f;
+            const F2 a2 = pack2(a, a), d2 = pack2(d, d);
+            F2 sum = pack2(0.0f, 0.0f);
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-                float e[2];
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                    float x = fmaf(__uint_as_float(v[16 * b + i + z]), a, d);
-                    if constexpr (MASK) {
-                        const int tok = tok0 + 32 * c + 16 * b + i + z;
-                        if (tok < r.lo || tok > r.hi) x = -INFINITY;
-                    }
-                    e[z] = ex2(x);
+                float2 x = both(fma2(pack2(__uint_as_float(v[16 * b + i]), __uint_as_float(v[16 * b + i + 1])), a2, d2));
+                if constexpr (MASK) {
+                    const int tok = tok0 + 32 * c + 16 * b + i;
+                    if (tok < r.lo || tok > r.hi) x.x = -INFINITY;
+                    if (tok + 1 < r.lo || tok + 1 > r.hi) x.y = -INFINITY;
                 }
-                sum += e[0] + e[1];
-                p[8 * b + i / 2] = pack_half(e[0], e[1]);
+                x.x = ex2(x.x);
+                x.y = ex2(x.y);
+                sum = add2(sum, pack2(x.x, x.y));
+                p[8 * b + i / 2] = pack_half(x.x, x.y);
             }
+            const float one = both(sum).x + both(sum).y;
             // a block without a visible token takes nothing from its scale, be it NaN
-            if (!MASK || sum != 0.0f) r.l = fmaf(sum, g.z, r.l);
+            if (!MASK || one != 0.0f) r.l = fmaf(one, g.z, r.l);
         }
-        // P's column 16 c lies on S's columns that are done
+        // P's columns 16 c .. lie on columns of S that are done
         tmem_store16(s_at + 16 * c, p);
+    };
+#pragma unroll 1
+    for (int c = 0; c < 4; c += 2) {
+        tmem_wait_load();
+        tmem_load32(s_at + 32 * (c + 1), v1);
+        weights(v0, c);
+        tmem_wait_load();
+        if (c == 0) tmem_load32(s_at + 64, v0);
+        weights(v1, c + 1);
     }
     tmem_wait_store();
+}
+
+// The steps of a task for a warp's 32 rows.  Not inlined: the state of the walk over
+// the tasks would take the registers that S needs.
+template <int D>
+__device__ __noinline__ bool softmax_rows(RowState &row, const RowPlace &at, const float4 (*scale)[8], bool ok) {
+    RowState r = row;
+    const RowPlace a = at;
+#pragma unroll 1
+    for (uint32_t j = 0; j < a.steps; ++j) {
+        const uint32_t n = a.it + j;
+        bar_wait(a.s_full, (a.parity + j) & 1, ok);
+        bar_wait(a.sc_full + 8 * (n & 3), (n >> 2) & 1, ok);  // at most one phase ahead once S is there
+        fence_after();
+        const int tok0 = a.tok0 + (int)j * kTileTokens;
+        if (tok0 >= a.all_lo && tok0 + kTileTokens - 1 <= a.all_hi)
+            softmax_step<D, false>(r, scale[n & 3], a.s_at, a.o_at, tok0, j == 0);
+        else
+            softmax_step<D, true>(r, scale[n & 3], a.s_at, a.o_at, tok0, j == 0);
+        fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) bar_arrive(a.p_full);
+    }
+    row = r;
+    return ok;
+}
+
+// ------------------------------------------------------------ loading
+
+struct LoadPlace {
+    uint8_t *k, *v;                              // two stages each
+    float4 (*scale)[8];
+    uint32_t k_full, k_empty, v_full, v_empty, sc_full;
+    uint32_t steps, it;
+    int begin, s, h, lo, hi;                     // first step; sequence, head and its visible 16-token blocks
+};
+
+// K and V of a task's steps, from 8-bit tiles to f16 operands (the loading warps)
+template <int D, int FMT>
+__device__ __noinline__ bool load_steps(const AttnArgs &A, const LoadPlace &place, bool ok) {
+    const LoadPlace P = place;
+    const int u = threadIdx.x - 32 * (kTileMmaWarp - kTileLoadWarps), lane = threadIdx.x & 31;
+    constexpr int PIECES = D / 16;                      // 16 codes each, of a token
+    constexpr int STEP = kTileLoaders / PIECES;         // tokens from piece to piece of a thread
+    constexpr int N = (kTileTokens + STEP - 1) / STEP;  // pieces of a thread, K or V of a step
+    constexpr int STAGE = TileSmem<D>::STAGE;
+    const int ch = u % PIECES, tk = u / PIECES;
+    const uint32_t odd = (ch >> 2) & 1;
+    uint4 kr[N], vr[N];
+    unsigned long long mine = 0;  // lane i < 8: the tile of block i of the step to be read, or 0: zeros
+    float2 head = make_float2(0.0f, 0.0f);
+    auto find = [&](int step) {
+        const int blk = step * 8 + (lane & 7);
+        mine = blk >= P.lo && blk < P.hi ? (unsigned long long)tile_of(A.c, A.b, P.s, P.h, blk) : 0ull;
+    };
+    auto load = [&](uint4(&r)[N], int z) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int t = tk + i * STEP;
+            const uint8_t *p = (const uint8_t *)__shfl_sync(0xffffffffu, mine, t >> 4);
+            r[i] = make_uint4(0, 0, 0, 0);
+            if (t < kTileTokens && p != nullptr)
+                r[i] = *reinterpret_cast<const uint4 *>(p + kHeader + (z * kBlock + (t & 15)) * D + 16 * ch);
+        }
+    };
+    auto put = [&](uint8_t *stage, const uint4(&r)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int t = tk + i * STEP;
+            if (t >= kTileTokens) break;
+            const uint32_t wd[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+            uint32_t h[8];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const uint32_t y = FMT == Q4RDNA_KV_INT8 ? wd[z] ^ 0x80808080u : wd[z];
+                h[2 * z] = pair_of<FMT, 0>(y);
+                h[2 * z + 1] = pair_of<FMT, 2>(y);
+            }
+            // the two halves in an order that keeps a phase's lanes in different banks
+            uint8_t *const to = stage + swizzled(t, 2 * ch + odd);
+            uint8_t *const too = stage + swizzled(t, 2 * ch + (odd ^ 1));
+            const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
+            *reinterpret_cast<uint4 *>(to) = odd ? b : a;
+            *reinterpret_cast<uint4 *>(too) = odd ? a : b;
+        }
+        fence_async();
+        __syncwarp();
+    };
+    find(P.begin);
+    load(kr, 0);
+    load(vr, 1);
+#pragma unroll 1
+    for (uint32_t j = 0; j < P.steps; ++j) {
+        const uint32_t n = P.it + j, stage = n & 1, parity = ((n >> 1) & 1) ^ 1;
+        if (u < 8) head = mine != 0 ? *reinterpret_cast<const float2 *>(mine) : make_float2(0.0f, 0.0f);
+        bar_wait(P.k_empty + 8 * stage, parity, ok);
+        put(P.k + stage * STAGE, kr);
+        if (lane == 0) bar_arrive(P.k_full + 8 * stage);
+        if (u < 32) {
+            if (u < 8) {
+                constexpr float M = FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f;  // e4m3 numbers come as 2^-8 of theirs
+                const float sv = head.y <= kTinyScale ? kTinyScale : head.y * M;  // NaN stays
+                P.scale[n & 3][u] = make_float4(head.x * M, log2f(sv), 1.0f / sv, 0.0f);
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(P.sc_full + 8 * (n & 3));
+        }
+        if (j + 1 < P.steps) {
+            find(P.begin + (int)j + 1);
+            load(kr, 0);
+        }
+        bar_wait(P.v_empty + 8 * stage, parity, ok);
+        put(P.v + stage * STAGE, vr);
+        if (lane == 0) bar_arrive(P.v_full + 8 * stage);
+        if (j + 1 < P.steps) load(vr, 1);
+    }
+    return ok;
 }
 
 template <int D, int FMT>
@@ -349,24 +491,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                     r.scale = steps > 0 ? sm.qscale[x][rt] : 0.0f;  // written by this warp
                     r.hi = there ? first + col / A.group : INT_MAX;  // (a padded row is computed and never read)
                     r.lo = there && A.window > 0 ? max(0, r.hi - A.window + 1) : 0;
-                    // tokens that all rows of the warp see
-                    const int all_lo = __reduce_max_sync(0xffffffffu, r.lo), all_hi = __reduce_min_sync(0xffffffffu, r.hi);
                     const uint32_t lanes = (uint32_t)(32 * (w & 3)) << 16;
-                    const uint32_t s_at = tmem + lanes + 128 * x, o_at = tmem + lanes + 256 + 128 * x;
-                    for (int j = 0; j < steps; ++j) {
-                        const uint32_t n = it + j;
-                        bar_wait(s_full(x), st[x] & 1, ok);
-                        bar_wait(sc_full(n & 3), (n >> 2) & 1, ok);  // at most one phase ahead once S is there
-                        ++st[x];
-                        fence_after();
-                        const int tok0 = (W.begin + j) * kTileTokens;
-                        if (tok0 >= all_lo && tok0 + kTileTokens - 1 <= all_hi)
-                            softmax_step<false>(r, sm.scale[n & 3], s_at, o_at, D, tok0, j == 0);
-                        else
-                            softmax_step<true>(r, sm.scale[n & 3], s_at, o_at, D, tok0, j == 0);
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(p_full(x));
+                    const uint32_t o_at = tmem + lanes + 256 + 128 * x;
+                    if (steps > 0) {
+                        RowPlace at;
+                        at.s_at = tmem + lanes + 128 * x;
+                        at.o_at = o_at;
+                        at.s_full = s_full(x);
+                        at.p_full = p_full(x);
+                        at.sc_full = sc_full(0);
+                        at.steps = steps;
+                        at.it = it;
+                        at.parity = st[x];
+                        at.tok0 = W.begin * kTileTokens;
+                        at.all_lo = __reduce_max_sync(0xffffffffu, r.lo);
+                        at.all_hi = __reduce_min_sync(0xffffffffu, r.hi);
+                        ok = softmax_rows<D>(r, at, sm.scale, ok);
+                        st[x] += steps;
                     }
                     // the result
                     if (steps > 0) bar_wait(o_full(x), tt[x] & 1, ok);
@@ -407,88 +548,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                 }
             } else if (w < kTileMmaWarp) {
                 // ------------------------------------------------ loading
-                const int u = threadIdx.x - 256;
-                constexpr int PIECES = D / 16;                             // 16 codes each, of a token
-                constexpr int STEP = kTileLoaders / PIECES;                // tokens from piece to piece of a thread
-                constexpr int N = (kTileTokens + STEP - 1) / STEP;         // pieces of a thread, K or V of a step
-                const int ch = u % PIECES, tk = u / PIECES;
-                // 16-token blocks that a column of the task sees
-                const Span sp = span_of(sq, W.col0, kTileCols, A.group, A.window, 4);
-                auto tile_at = [&](int blk) -> const uint8_t * {  // null: nothing to read, zeros
-                    return blk >= sp.lo && blk < sp.hi ? tile_of(A.c, B, W.s, W.h, blk) : nullptr;
-                };
-                uint4 kr[N], vr[N];
-                const uint8_t *at[N];
-                auto find = [&](int step) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        at[i] = tk + i * STEP < kTileTokens ? tile_at(step * 8 + (tk + i * STEP) / 16) : nullptr;
-                    }
-                };
-                auto load = [&](uint4(&r)[N], int z) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const int t = (tk + i * STEP) & 15;
-                        r[i] = at[i] == nullptr ? make_uint4(0, 0, 0, 0)
-                                                : *reinterpret_cast<const uint4 *>(at[i] + kHeader + (z * kBlock + t) * D + 16 * ch);
-                    }
-                };
-                auto put = [&](uint8_t *stage, const uint4(&r)[N]) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const int t = tk + i * STEP;
-                        if (t >= kTileTokens) break;
-                        const uint32_t wd[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-                        uint32_t h[8];
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const uint32_t y = FMT == Q4RDNA_KV_INT8 ? wd[z] ^ 0x80808080u : wd[z];
-                            h[2 * z] = pair_of<FMT, 0>(y);
-                            h[2 * z + 1] = pair_of<FMT, 2>(y);
-                        }
-                        // the two halves in an order that keeps a phase's lanes in different banks
-                        const bool odd = (ch >> 2) & 1;
-                        const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
-                        *reinterpret_cast<uint4 *>(stage + swizzled(t, 2 * ch + (odd ? 1 : 0))) = odd ? b : a;
-                        *reinterpret_cast<uint4 *>(stage + swizzled(t, 2 * ch + (odd ? 0 : 1))) = odd ? a : b;
-                    }
-                    fence_async();
-                    __syncwarp();
-                };
                 if (steps > 0) {
-                    find(W.begin);
-                    load(kr, 0);
-                    load(vr, 1);
-                }
-                for (int j = 0; j < steps; ++j) {
-                    const uint32_t n = it + j;
-                    const int stage = n & 1;
-                    const uint32_t parity = ((n >> 1) & 1) ^ 1;
-                    float2 hd = make_float2(0.0f, 0.0f);
-                    if (w == 8 && lane < 8) {
-                        const uint8_t *t = tile_at((W.begin + j) * 8 + lane);
-                        if (t != nullptr) hd = *reinterpret_cast<const float2 *>(t);
-                    }
-                    bar_wait(k_empty(stage), parity, ok);
-                    put(sm.k[stage], kr);
-                    if (lane == 0) bar_arrive(k_full(stage));
-                    if (w == 8) {
-                        if (lane < 8) {
-                            constexpr float M = FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f;  // e4m3 numbers come as 2^-8 of theirs
-                            const float sv = hd.y <= kTinyScale ? kTinyScale : hd.y * M;  // NaN stays
-                            sm.scale[n & 3][lane] = make_float4(hd.x * M, log2f(sv), 1.0f / sv, 0.0f);
-                        }
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(sc_full(n & 3));
-                    }
-                    if (j + 1 < steps) {
-                        find(W.begin + j + 1);
-                        load(kr, 0);
-                    }
-                    bar_wait(v_empty(stage), parity, ok);
-                    put(sm.v[stage], vr);
-                    if (lane == 0) bar_arrive(v_full(stage));
-                    if (j + 1 < steps) load(vr, 1);
+                    // 16-token blocks that a column of the task sees
+                    const Span sp = span_of(sq, W.col0, kTileCols, A.group, A.window, 4);
+                    LoadPlace p;
+                    p.k = sm.k[0];
+                    p.v = sm.v[0];
+                    p.scale = sm.scale;
+                    p.k_full = k_full(0);
+                    p.k_empty = k_empty(0);
+                    p.v_full = v_full(0);
+                    p.v_empty = v_empty(0);
+                    p.sc_full = sc_full(0);
+                    p.steps = steps;
+                    p.it = it;
+                    p.begin = W.begin;
+                    p.s = W.s;
+                    p.h = W.h;
+                    p.lo = sp.lo;
+                    p.hi = sp.hi;
+                    ok = load_steps<D, FMT>(A, p, ok);
                 }
             } else if (lane == 0) {
                 // ------------------------------------------------ products
