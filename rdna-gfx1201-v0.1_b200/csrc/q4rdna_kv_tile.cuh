@@ -17,9 +17,9 @@
 //   * While one tile's softmax runs, the other tile's products do.
 //   * Scales: a block's key scale multiplies its 16 columns of S, the logarithm of its
 //     value scale joins the exponent, p = 2^(s + log2 sv - R); the sum of the weights
-//     themselves takes each block's sum times 1 / sv.  R, per row, moves only when an
-//     exponent outgrows it by 8 (the row's O is then rescaled by its own thread), and p
-//     carries 2^7: f16 holds weights from 2^15 to 2^-24.
+//     themselves takes each block's sum times 1 / sv.  R, per row, moves only when the
+//     weights would leave f16's range (the row's O is then rescaled by its own thread),
+//     and p carries 2^7.
 //   * Tensor memory (512 columns): S0 S1 O0 O1, 128 each.
 // Every wait is bounded (about a second, %globaltimer): on expiry the role sets bit 4
 // of the fault word and takes no more waits, copies or products; the issuing thread
@@ -124,16 +124,16 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(addr));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];\n"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
+}
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-        "%14, %15};" ::"r"(v[0]),
-        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
@@ -166,104 +166,98 @@ struct RowPlace {
     int tok0, all_lo, all_hi;           // first token of the task; tokens that all rows of the warp see
 };
 
-// One step of one row: S to P.  MASK: some row of the warp does not see all of it.
-// S is read twice, 32 columns ahead of the arithmetic, rather than held (128 registers).
+// One step of one row: S to P in one pass over S with the reference as it stands: p is
+// right for any reference, as long as it stays in f16's range, and no weight is above
+// the sum of its block.  Where a sum is above 2^15 (or the row has seen nothing yet) the
+// step's largest exponent is looked for, becomes the reference, and the pass is made
+// again; P goes to tensor memory (over S) only when it is right.
+// MASK: some row of the warp does not see all of the step.
 template <int D, bool MASK>
 __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, uint32_t s_at, uint32_t o_at, int tok0,
                                              bool first) {
-    uint32_t v0[32], v1[32];
-    // columns 32 c .. of S: the largest exponent
-    float t = -INFINITY;
-    auto largest = [&](const uint32_t(&v)[32], int c) {
+    uint32_t p[64];
+    float add;
+    bool look = first;
+#pragma unroll 1
+    while (true) {
+        if (look) {
+            uint32_t v[32];
+            float t = -INFINITY;  // the largest exponent
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                tmem_load32(s_at + 32 * c, v);
+                tmem_wait_load();
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const float4 f = scale[2 * c + b];
-            float m[2] = {-INFINITY, -INFINITY};
+                for (int b = 0; b < 2; ++b) {
+                    const float4 f = scale[2 * c + b];
+                    float m = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                float x[2];
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                    x[z] = __uint_as_float(v[16 * b + i + z]);
-                    if constexpr (MASK) {
-                        const int tok = tok0 + 32 * c + 16 * b + i + z;
-                        if (tok < r.lo || tok > r.hi) x[z] = -INFINITY;
+                    for (int i = 0; i < 16; ++i) {
+                        float x = __uint_as_float(v[16 * b + i]);
+                        if constexpr (MASK) {
+                            const int tok = tok0 + 32 * c + 16 * b + i;
+                            if (tok < r.lo || tok > r.hi) x = -INFINITY;
+                        }
+                        m = fmaxf(m, x);
                     }
+                    // a block without a visible token has m = -inf, which a scale of 0 would turn into NaN
+                    if (!MASK || m != -INFINITY) t = fmaxf(t, fmaf(m, f.x * r.scale, f.y));
                 }
-                m[i / 2 & 1] = fmaxf(fmaxf(m[i / 2 & 1], x[0]), x[1]);
             }
-            const float mx = fmaxf(m[0], m[1]), y = fmaf(mx, f.x * r.scale, f.y);
-            // a block without a visible token has mx = -inf, which a scale of 0 would turn into NaN
-            t = fmaxf(t, MASK && mx == -INFINITY ? -INFINITY : y);
+            const float f = t > r.R ? ex2(r.R - t) : 1.0f;  // 0 for the first: R = -inf
+            if (t > r.R) r.R = t;
+            r.l *= f;
+            if (!first) {
+                // the products of the step before have ended (they come before this S), the next ones wait for this P
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    tmem_load32(o_at + c, v);
+                    tmem_wait_load();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                    tmem_store32(o_at + c, v);
+                }
+            }
         }
-    };
-    tmem_load32(s_at, v0);
-#pragma unroll 1
-    for (int c = 0; c < 4; c += 2) {
-        tmem_wait_load();
-        tmem_load32(s_at + 32 * (c + 1), v1);
-        largest(v0, c);
-        tmem_wait_load();
-        tmem_load32(s_at + 32 * ((c + 2) & 3), v0);  // at the end the next pass's first
-        largest(v1, c + 1);
-    }
-    float f = 1.0f;
-    const bool moved = t > r.R + 8.0f;  // also the first: R = -inf
-    if (moved) {
-        f = ex2(r.R - t);
-        r.R = t;
-        r.l *= f;
-    }
-    if (__any_sync(0xffffffffu, moved) && !first) {
-        // the products of the step before have ended (they come before this S), the next ones wait for this P
-        tmem_wait_load();
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-            tmem_load32(o_at + c, v1);
+        const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
+        uint32_t v[2][16];
+        tmem_load16(s_at, v[0]);
+        add = 0.0f;
+        float most = 0.0f;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
             tmem_wait_load();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v1[i] = __float_as_uint(__uint_as_float(v1[i]) * f);
-            tmem_store32(o_at + c, v1);
-        }
-    }
-    const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
-    auto weights = [&](const uint32_t(&v)[32], int c) {
-        uint32_t p[16];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const float4 g = scale[2 * c + b];
+            if (b < 7) tmem_load16(s_at + 16 * (b + 1), v[(b + 1) & 1]);
+            const float4 g = scale[b];
             const float a = g.x * r.scale, d = g.y - ref;
             const F2 a2 = pack2(a, a), d2 = pack2(d, d);
-            F2 sum = pack2(0.0f, 0.0f);
+            F2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-                float2 x = both(fma2(pack2(__uint_as_float(v[16 * b + i]), __uint_as_float(v[16 * b + i + 1])), a2, d2));
+                float2 x = both(fma2(pack2(__uint_as_float(v[b & 1][i]), __uint_as_float(v[b & 1][i + 1])), a2, d2));
                 if constexpr (MASK) {
-                    const int tok = tok0 + 32 * c + 16 * b + i;
+                    const int tok = tok0 + 16 * b + i;
                     if (tok < r.lo || tok > r.hi) x.x = -INFINITY;
                     if (tok + 1 < r.lo || tok + 1 > r.hi) x.y = -INFINITY;
                 }
                 x.x = ex2(x.x);
                 x.y = ex2(x.y);
-                sum = add2(sum, pack2(x.x, x.y));
+                sum[i / 2 & 1] = add2(sum[i / 2 & 1], pack2(x.x, x.y));
                 p[8 * b + i / 2] = pack_half(x.x, x.y);
             }
-            const float one = both(sum).x + both(sum).y;
+            const float2 both_sums = both(add2(sum[0], sum[1]));
+            const float one = both_sums.x + both_sums.y;
+            most = fmaxf(most, one);
             // a block without a visible token takes nothing from its scale, be it NaN
-            if (!MASK || one != 0.0f) r.l = fmaf(one, g.z, r.l);
+            if (!MASK || one != 0.0f) add = fmaf(one, g.z, add);
         }
-        // P's columns 16 c .. lie on columns of S that are done
-        tmem_store16(s_at + 16 * c, p);
-    };
-#pragma unroll 1
-    for (int c = 0; c < 4; c += 2) {
-        tmem_wait_load();
-        tmem_load32(s_at + 32 * (c + 1), v1);
-        weights(v0, c);
-        tmem_wait_load();
-        if (c == 0) tmem_load32(s_at + 64, v0);
-        weights(v1, c + 1);
+        if (look) break;  // every exponent is now at most the reference
+        look = __any_sync(0xffffffffu, most > 32768.0f || r.R == -INFINITY);
+        if (!look) break;
     }
+    r.l += add;
+    tmem_store32(s_at, *reinterpret_cast<uint32_t(*)[32]>(p));
+    tmem_store32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
     tmem_wait_store();
 }
 
@@ -384,26 +378,98 @@ __device__ __noinline__ bool load_steps(const AttnArgs &A, const LoadPlace &plac
     return ok;
 }
 
+// ------------------------------------------------------------ products
+
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
+
+// Barriers of the CTA: K and V stage full / empty, scales (ring of 4), and per tile Q
+// written, S computed, P written, O complete
+struct Bars {
+    uint32_t at;
+    __device__ __forceinline__ uint32_t k_full(int i) const { return at + 8u * i; }
+    __device__ __forceinline__ uint32_t k_empty(int i) const { return at + 8u * (2 + i); }
+    __device__ __forceinline__ uint32_t v_full(int i) const { return at + 8u * (4 + i); }
+    __device__ __forceinline__ uint32_t v_empty(int i) const { return at + 8u * (6 + i); }
+    __device__ __forceinline__ uint32_t sc_full(int i) const { return at + 8u * (8 + i); }
+    __device__ __forceinline__ uint32_t q_full(int x) const { return at + 8u * (12 + x); }
+    __device__ __forceinline__ uint32_t s_full(int x) const { return at + 8u * (14 + x); }
+    __device__ __forceinline__ uint32_t p_full(int x) const { return at + 8u * (16 + x); }
+    __device__ __forceinline__ uint32_t o_full(int x) const { return at + 8u * (18 + x); }
+    __device__ __forceinline__ uint32_t drained() const { return at + 8u * 20; }
+};
+
+// The products of a task's steps.  Order: S0 S1 of the first step, then per step and
+// tile O += P V and the next step's S.  st, tt: steps and tasks of either tile so far.
+template <int D>
+__device__ __forceinline__ void issue_steps(TileSmem<D> &sm, uint32_t tmem, Bars bar, int steps, uint32_t it, int tiles,
+                                            const uint32_t (&st)[2], const uint32_t (&tt)[2], bool &ok) {
+    using Smem = TileSmem<D>;
+    // f16 operands, f32 sums, M = 128; S: both K-major, N = 128; O: B MN-major, N = D
+    constexpr uint32_t S_DESC = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | (8u << 24);
+    constexpr uint32_t O_DESC = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+    const uint64_t q0 = operand(smem_u32(sm.q[0]), 16), k0 = operand(smem_u32(sm.k[0]), 16);
+    const uint64_t v0 = operand(smem_u32(sm.v[0]), Smem::PANEL);
+    auto scores = [&](int x, uint32_t stage) {
+        const uint64_t a = q0 + x * (Smem::STAGE >> 4), b = k0 + stage * (Smem::STAGE >> 4);
+        if (elected()) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const uint32_t off = ((i >> 2) * Smem::PANEL + (i & 3) * 32) >> 4;
+                mma_ss(tmem + 128 * x, a + off, b + off, S_DESC, i > 0);
+            }
+            commit(bar.s_full(x));
+        }
+        __syncwarp();
+    };
+    auto release = [&](uint32_t which) {
+        if (elected()) commit(which);
+        __syncwarp();
+    };
+    for (int x = 0; x < tiles; ++x) bar_wait(bar.q_full(x), tt[x] & 1, ok);
+    bar_wait(bar.k_full(it & 1), (it >> 1) & 1, ok);
+    fence_after();
+    if (ok) {
+        for (int x = 0; x < tiles; ++x) scores(x, it & 1);
+        release(bar.k_empty(it & 1));
+    }
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j) {
+        const uint32_t n = it + j;
+        if (j + 1 < steps) bar_wait(bar.k_full((n + 1) & 1), ((n + 1) >> 1) & 1, ok);
+        bar_wait(bar.v_full(n & 1), (n >> 1) & 1, ok);
+        const uint64_t b = v0 + (n & 1) * (Smem::STAGE >> 4);
+#pragma unroll 1
+        for (int x = 0; x < tiles; ++x) {
+            bar_wait(bar.p_full(x), (st[x] + j) & 1, ok);
+            fence_after();
+            if (!ok) continue;
+            if (elected()) {
+#pragma unroll
+                for (int i = 0; i < kTileTokens / 16; ++i)
+                    mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * i, b + i * (2048 >> 4), O_DESC, j > 0 || i > 0);
+                if (j + 1 == steps) commit(bar.o_full(x));
+            }
+            __syncwarp();
+            if (j + 1 < steps) scores(x, (n + 1) & 1);
+        }
+        if (ok) {
+            release(bar.v_empty(n & 1));
+            if (j + 1 < steps) release(bar.k_empty((n + 1) & 1));
+        }
+    }
+}
+
 template <int D, int FMT>
 __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_constant__ AttnArgs A) {
     using Smem = TileSmem<D>;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
-    const Batch &B = A.b;
+    extern __shared__ __align__(1024) uint8_t tile_smem[];
+    Smem &sm = *reinterpret_cast<Smem *>(tile_smem);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t bar0 = smem_u32(sm.bar);
-    // mbarriers: K and V stage full / empty, scales (ring of 4), and per tile Q written, S
-    // computed, P written, O complete
-    auto k_full = [&](int i) { return bar0 + 8u * i; };
-    auto k_empty = [&](int i) { return bar0 + 8u * (2 + i); };
-    auto v_full = [&](int i) { return bar0 + 8u * (4 + i); };
-    auto v_empty = [&](int i) { return bar0 + 8u * (6 + i); };
-    auto sc_full = [&](int i) { return bar0 + 8u * (8 + i); };
-    auto q_full = [&](int x) { return bar0 + 8u * (12 + x); };
-    auto s_full = [&](int x) { return bar0 + 8u * (14 + x); };
-    auto p_full = [&](int x) { return bar0 + 8u * (16 + x); };
-    auto o_full = [&](int x) { return bar0 + 8u * (18 + x); };
-    const uint32_t drained = bar0 + 8u * 20;
+    const Bars bar{smem_u32(sm.bar)};
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (w == kTileMmaWarp) {
@@ -413,17 +479,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            bar_init(k_full(i), kTileLoadWarps);
-            bar_init(v_full(i), kTileLoadWarps);
-            bar_init(k_empty(i), 1);
-            bar_init(v_empty(i), 1);
-            bar_init(q_full(i), 4);
-            bar_init(s_full(i), 1);
-            bar_init(p_full(i), 4);
-            bar_init(o_full(i), 1);
+            bar_init(bar.k_full(i), kTileLoadWarps);
+            bar_init(bar.v_full(i), kTileLoadWarps);
+            bar_init(bar.k_empty(i), 1);
+            bar_init(bar.v_empty(i), 1);
+            bar_init(bar.q_full(i), 4);
+            bar_init(bar.s_full(i), 1);
+            bar_init(bar.p_full(i), 4);
+            bar_init(bar.o_full(i), 1);
         }
-        for (int i = 0; i < 4; ++i) bar_init(sc_full(i), 1);
-        bar_init(drained, 1);
+        for (int i = 0; i < 4; ++i) bar_init(bar.sc_full(i), 1);
+        bar_init(bar.drained(), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     fence_before();
@@ -481,7 +547,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                         }
                         fence_async();
                         __syncwarp();
-                        if (lane == 0) bar_arrive(q_full(x));
+                        if (lane == 0) bar_arrive(bar.q_full(x));
                     }
                     RowState r;
                     const int col = W.col0 + kTileRows * x + rt;
@@ -497,9 +563,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                         RowPlace at;
                         at.s_at = tmem + lanes + 128 * x;
                         at.o_at = o_at;
-                        at.s_full = s_full(x);
-                        at.p_full = p_full(x);
-                        at.sc_full = sc_full(0);
+                        at.s_full = bar.s_full(x);
+                        at.p_full = bar.p_full(x);
+                        at.sc_full = bar.sc_full(0);
                         at.steps = steps;
                         at.it = it;
                         at.parity = st[x];
@@ -510,7 +576,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                         st[x] += steps;
                     }
                     // the result
-                    if (steps > 0) bar_wait(o_full(x), tt[x] & 1, ok);
+                    if (steps > 0) bar_wait(bar.o_full(x), tt[x] & 1, ok);
                     if (steps > 0) ++tt[x];
                     fence_after();
                     const bool whole = W.whole();
@@ -555,11 +621,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                     p.k = sm.k[0];
                     p.v = sm.v[0];
                     p.scale = sm.scale;
-                    p.k_full = k_full(0);
-                    p.k_empty = k_empty(0);
-                    p.v_full = v_full(0);
-                    p.v_empty = v_empty(0);
-                    p.sc_full = sc_full(0);
+                    p.k_full = bar.k_full(0);
+                    p.k_empty = bar.k_empty(0);
+                    p.v_full = bar.v_full(0);
+                    p.v_empty = bar.v_empty(0);
+                    p.sc_full = bar.sc_full(0);
                     p.steps = steps;
                     p.it = it;
                     p.begin = W.begin;
@@ -569,51 +635,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                     p.hi = sp.hi;
                     ok = load_steps<D, FMT>(A, p, ok);
                 }
-            } else if (lane == 0) {
+            } else {
                 // ------------------------------------------------ products
-                // f16 operands, f32 sums, M = 128; S: both K-major, N = 128; O: B MN-major, N = D
-                constexpr uint32_t S_DESC = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | (8u << 24);
-                constexpr uint32_t O_DESC = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
-                auto scores = [&](int x, int stage) {
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const uint32_t off = (i >> 2) * Smem::PANEL + (i & 3) * 32;
-                        mma_ss(tmem + 128 * x, operand(smem_u32(sm.q[x]) + off, 16), operand(smem_u32(sm.k[stage]) + off, 16),
-                               S_DESC, i > 0);
-                    }
-                    commit(s_full(x));
-                };
+                // The whole warp walks and waits; one elected lane issues, so that operands
+                // stay in uniform registers.
                 if (steps > 0) {
-                    for (int x = 0; x < tiles; ++x) bar_wait(q_full(x), tt[x] & 1, ok);
-                    bar_wait(k_full(it & 1), (it >> 1) & 1, ok);
-                    fence_after();
-                    if (ok) {
-                        for (int x = 0; x < tiles; ++x) scores(x, it & 1);
-                        commit(k_empty(it & 1));
-                    }
-                }
-                for (int j = 0; j < steps; ++j) {
-                    const uint32_t n = it + j;
-                    if (j + 1 < steps) bar_wait(k_full((n + 1) & 1), ((n + 1) >> 1) & 1, ok);
-                    bar_wait(v_full(n & 1), (n >> 1) & 1, ok);
+                    issue_steps<D>(sm, tmem, bar, steps, it, tiles, st, tt, ok);
                     for (int x = 0; x < tiles; ++x) {
-                        bar_wait(p_full(x), st[x] & 1, ok);
-                        ++st[x];
-                        fence_after();
-                        if (!ok) continue;
-#pragma unroll
-                        for (int i = 0; i < kTileTokens / 16; ++i)
-                            mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * i,
-                                   operand(smem_u32(sm.v[n & 1]) + i * 2048, Smem::PANEL), O_DESC, j > 0 || i > 0);
-                        if (j + 1 == steps) commit(o_full(x));
-                        else scores(x, (n + 1) & 1);
-                    }
-                    if (ok) {
-                        commit(v_empty(n & 1));
-                        if (j + 1 < steps) commit(k_empty((n + 1) & 1));
+                        ++tt[x];
+                        st[x] += steps;
                     }
                 }
-                for (int x = 0; x < tiles && steps > 0; ++x) ++tt[x];
             }
             it += steps;
             if (W.open()) {
@@ -623,10 +655,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
         }
     }
     if (threadIdx.x == 0 && !open) A.rec[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (w == kTileMmaWarp && lane == 0) {  // no product may still run when the tensor memory goes
+    if (w == kTileMmaWarp) {  // no product may still run when the tensor memory goes
         bool last = true;
-        commit(drained);
-        bar_wait(drained, 0, last);
+        if (elected()) commit(bar.drained());
+        __syncwarp();
+        bar_wait(bar.drained(), 0, last);
     }
     fence_before();
     __syncthreads();
