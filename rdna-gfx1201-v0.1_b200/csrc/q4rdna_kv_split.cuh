@@ -49,14 +49,31 @@ __device__ __forceinline__ Span span_of(const Seq &q, int col0, int nc, int grou
 // Work of a task: one piece at least, so that every task lies in a share and its rows are written
 __device__ __forceinline__ int work_of(const Span &s) { return max(1, s.hi - s.lo); }
 
-// Work of one kv head of a sequence; 0 for a sequence that is not this kernel's
+// Work of one kv head of a sequence; 0 for a sequence that is not this kernel's.  The
+// lanes of a warp call it together, each with a sequence of its own or all with the
+// same one; a sequence of many tasks is summed by the whole warp.
 __device__ __forceinline__ long long head_work(const AttnArgs &A, const Seq &q, int nc, int shift) {
+    const int lane = threadIdx.x & 31;
     const int cols = q.n * A.group;
-    if (cols < A.few || cols >= A.many) return 0;
-    if (nc >= cols) return cols == 0 ? 0 : work_of(span_of(q, 0, nc, A.group, A.window, shift));
-    long long w = 0;
-    for (int c = 0; c < cols; c += nc) w += work_of(span_of(q, c, nc, A.group, A.window, shift));
-    return w;
+    const bool ours = cols >= A.few && cols < A.many && cols > 0;
+    long long mine = ours && cols <= nc ? work_of(span_of(q, 0, nc, A.group, A.window, shift)) : 0;
+    unsigned todo = __ballot_sync(0xffffffffu, ours && cols > nc);
+    while (todo != 0) {
+        const int who = __ffs(todo) - 1;
+        Seq x;
+        x.a = 0;
+        x.n = __shfl_sync(0xffffffffu, q.n, who);
+        x.L = __shfl_sync(0xffffffffu, q.L, who);
+        // (lanes with the same sequence are served at once)
+        const bool same = x.n == q.n && x.L == q.L && ours && cols > nc;
+        long long w = 0;
+        for (int c = lane * nc; c < x.n * A.group; c += 32 * nc) w += work_of(span_of(x, c, nc, A.group, A.window, shift));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        if (same) mine = w;
+        todo &= ~__ballot_sync(0xffffffffu, same);
+    }
+    return mine;
 }
 
 template <int WARPS>
@@ -74,7 +91,11 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
     constexpr int THREADS = 32 * WARPS;
     const Batch &B = A.b;
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto work = [&](int s) -> long long { return s < B.S ? head_work(A, load_seq(B, s), nc, shift) * A.c.hk : 0; };
+    auto work = [&](int s) -> long long {
+        Seq q{0, 0, 0};
+        if (s < B.S) q = load_seq(B, s);
+        return head_work(A, q, nc, shift) * A.c.hk;
+    };
     const long long first = work(threadIdx.x);  // of a chunk of THREADS sequences; most batches are one
     long long total = 0;
     for (int base = 0; base < B.S; base += THREADS) {
@@ -117,7 +138,8 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
     return min(share, total - begin);
 }
 
-// The tasks of a share, one after the other (the same in all threads)
+// The tasks of a share, one after the other (the same in all threads; the lanes of a
+// warp call next() together)
 struct Walk {
     const AttnArgs &A;
     int nc, shift;
@@ -152,11 +174,27 @@ struct Walk {
                     rest -= h * hw;
                 }
             }
-            span = span_of(q, col0, nc, A.group, A.window, shift);
-            all = work_of(span);
-            if (rest < all) break;
-            rest -= all;
-            col0 += nc;
+            // the task with `rest` in it: the warp looks at 32 tasks at a time
+            const int lane = threadIdx.x & 31;
+            const int c = col0 + lane * nc;
+            const int mine = c < cols ? work_of(span_of(q, c, nc, A.group, A.window, shift)) : 0;
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            const unsigned behind = __ballot_sync(0xffffffffu, upto > rest);
+            if (behind != 0) {
+                const int hit = __ffs(behind) - 1;
+                all = __shfl_sync(0xffffffffu, mine, hit);
+                rest -= __shfl_sync(0xffffffffu, upto, hit) - all;
+                col0 += hit * nc;
+                span = span_of(q, col0, nc, A.group, A.window, shift);
+                break;
+            }
+            rest -= __shfl_sync(0xffffffffu, upto, 31);
+            col0 += 32 * nc;
         }
         begin = span.lo + (int)rest;
         cnt = (int)min((long long)(all - (int)rest), left);

@@ -81,6 +81,18 @@ __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity) {
         }
     }
 }
+// Whether three phases are there, asked for at once (one barrier's answer takes about 100 cycles)
+__device__ __forceinline__ bool bar_try3(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p, q, r;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n"
+        " and.pred p, p, q;\n and.pred p, p, r;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(b0), "r"(p0), "r"(b1), "r"(p1), "r"(b2), "r"(p2)
+        : "memory");
+    return ok != 0;
+}
 // Waits for the phase of the given parity; `ok` false: not any more
 __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, bool &ok) {
     if (ok && !bar_try(bar, parity)) {
@@ -171,10 +183,11 @@ struct RowPlace {
 // the sum of its block.  Where a sum is above 2^15 (or the row has seen nothing yet) the
 // step's largest exponent is looked for, becomes the reference, and the pass is made
 // again; P goes to tensor memory (over S) only when it is right.
-// MASK: some row of the warp does not see all of the step.
-template <int D, bool MASK>
+// Tokens that a row of the warp does not see lie outside [all_lo, all_hi]; only the
+// blocks there pay for the mask.
+template <int D>
 __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, uint32_t s_at, uint32_t o_at, int tok0,
-                                             bool first) {
+                                             int all_lo, int all_hi, bool first) {
     uint32_t p[64];
     float add;
     bool look = first;
@@ -187,21 +200,20 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
             for (int c = 0; c < 4; ++c) {
                 tmem_load32(s_at + 32 * c, v);
                 tmem_wait_load();
+                const int tok = tok0 + 32 * c;
+                if (tok < all_lo || tok + 31 > all_hi) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (tok + i < r.lo || tok + i > r.hi) v[i] = 0xff800000u;  // -inf
+                }
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const float4 f = scale[2 * c + b];
                     float m = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float x = __uint_as_float(v[16 * b + i]);
-                        if constexpr (MASK) {
-                            const int tok = tok0 + 32 * c + 16 * b + i;
-                            if (tok < r.lo || tok > r.hi) x = -INFINITY;
-                        }
-                        m = fmaxf(m, x);
-                    }
+                    for (int i = 0; i < 16; ++i) m = fmaxf(m, __uint_as_float(v[16 * b + i]));
                     // a block without a visible token has m = -inf, which a scale of 0 would turn into NaN
-                    if (!MASK || m != -INFINITY) t = fmaxf(t, fmaf(m, f.x * r.scale, f.y));
+                    if (m != -INFINITY) t = fmaxf(t, fmaf(m, f.x * r.scale, f.y));
                 }
             }
             const float f = t > r.R ? ex2(r.R - t) : 1.0f;  // 0 for the first: R = -inf
@@ -221,35 +233,51 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
         }
         const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
         uint32_t v[2][16];
+        float e[2][16];
         tmem_load16(s_at, v[0]);
         add = 0.0f;
         float most = 0.0f;
+        // the weights of a block in flight while the block before it is summed and packed
 #pragma unroll
-        for (int b = 0; b < 8; ++b) {
-            tmem_wait_load();
-            if (b < 7) tmem_load16(s_at + 16 * (b + 1), v[(b + 1) & 1]);
-            const float4 g = scale[b];
-            const float a = g.x * r.scale, d = g.y - ref;
-            const F2 a2 = pack2(a, a), d2 = pack2(d, d);
-            F2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+        for (int b = 0; b < 9; ++b) {
+            if (b < 8) {
+                tmem_wait_load();
+                if (b < 7) tmem_load16(s_at + 16 * (b + 1), v[(b + 1) & 1]);
+                const float4 g = scale[b];
+                const float a = g.x * r.scale, d = g.y - ref;
+                const F2 a2 = pack2(a, a), d2 = pack2(d, d);
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                float2 x = both(fma2(pack2(__uint_as_float(v[b & 1][i]), __uint_as_float(v[b & 1][i + 1])), a2, d2));
-                if constexpr (MASK) {
-                    const int tok = tok0 + 16 * b + i;
-                    if (tok < r.lo || tok > r.hi) x.x = -INFINITY;
-                    if (tok + 1 < r.lo || tok + 1 > r.hi) x.y = -INFINITY;
+                for (int i = 0; i < 16; i += 2) {
+                    const float2 x =
+                        both(fma2(pack2(__uint_as_float(v[b & 1][i]), __uint_as_float(v[b & 1][i + 1])), a2, d2));
+                    e[b & 1][i] = x.x;
+                    e[b & 1][i + 1] = x.y;
                 }
-                x.x = ex2(x.x);
-                x.y = ex2(x.y);
-                sum[i / 2 & 1] = add2(sum[i / 2 & 1], pack2(x.x, x.y));
-                p[8 * b + i / 2] = pack_half(x.x, x.y);
+                const int tok = tok0 + 16 * b;
+                if (tok < all_lo || tok + 15 > all_hi) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (tok + i < r.lo || tok + i > r.hi) e[b & 1][i] = -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) e[b & 1][i] = ex2(e[b & 1][i]);
             }
-            const float2 both_sums = both(add2(sum[0], sum[1]));
-            const float one = both_sums.x + both_sums.y;
-            most = fmaxf(most, one);
-            // a block without a visible token takes nothing from its scale, be it NaN
-            if (!MASK || one != 0.0f) add = fmaf(one, g.z, add);
+            if (b > 0) {
+                const float(&y)[16] = e[(b - 1) & 1];
+                F2 sum[2] = {pack2(y[0], y[1]), pack2(y[2], y[3])};
+#pragma unroll
+                for (int i = 4; i < 16; i += 4) {
+                    sum[0] = add2(sum[0], pack2(y[i], y[i + 1]));
+                    sum[1] = add2(sum[1], pack2(y[i + 2], y[i + 3]));
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) p[8 * (b - 1) + i / 2] = pack_half(y[i], y[i + 1]);
+                const float2 two = both(add2(sum[0], sum[1]));
+                const float one = two.x + two.y;
+                most = fmaxf(most, one);
+                // a block without a visible token takes nothing from its scale, be it NaN
+                if (one != 0.0f) add = fmaf(one, scale[b - 1].z, add);
+            }
         }
         if (look) break;  // every exponent is now at most the reference
         look = __any_sync(0xffffffffu, most > 32768.0f || r.R == -INFINITY);
@@ -274,10 +302,7 @@ __device__ __noinline__ bool softmax_rows(RowState &row, const RowPlace &at, con
         bar_wait(a.sc_full + 8 * (n & 3), (n >> 2) & 1, ok);  // at most one phase ahead once S is there
         fence_after();
         const int tok0 = a.tok0 + (int)j * kTileTokens;
-        if (tok0 >= a.all_lo && tok0 + kTileTokens - 1 <= a.all_hi)
-            softmax_step<D, false>(r, scale[n & 3], a.s_at, a.o_at, tok0, j == 0);
-        else
-            softmax_step<D, true>(r, scale[n & 3], a.s_at, a.o_at, tok0, j == 0);
+        softmax_step<D>(r, scale[n & 3], a.s_at, a.o_at, tok0, a.all_lo, a.all_hi, j == 0);
         fence_before();
         __syncwarp();
         if ((threadIdx.x & 31) == 0) bar_arrive(a.p_full);
@@ -439,26 +464,31 @@ __device__ __forceinline__ void issue_steps(TileSmem<D> &sm, uint32_t tmem, Bars
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
         const uint32_t n = it + j;
-        if (j + 1 < steps) bar_wait(bar.k_full((n + 1) & 1), ((n + 1) >> 1) & 1, ok);
-        bar_wait(bar.v_full(n & 1), (n >> 1) & 1, ok);
+        const bool more = j + 1 < steps;
+        const uint32_t kb = more ? bar.k_full((n + 1) & 1) : bar.v_full(n & 1), kp = more ? ((n + 1) >> 1) & 1 : (n >> 1) & 1;
+        if (!bar_try3(kb, kp, bar.v_full(n & 1), (n >> 1) & 1, bar.p_full(0), (st[0] + j) & 1)) {
+            bar_wait(kb, kp, ok);
+            bar_wait(bar.v_full(n & 1), (n >> 1) & 1, ok);
+            bar_wait(bar.p_full(0), (st[0] + j) & 1, ok);
+        }
         const uint64_t b = v0 + (n & 1) * (Smem::STAGE >> 4);
 #pragma unroll 1
         for (int x = 0; x < tiles; ++x) {
-            bar_wait(bar.p_full(x), (st[x] + j) & 1, ok);
+            if (x == 1) bar_wait(bar.p_full(1), (st[1] + j) & 1, ok);
             fence_after();
             if (!ok) continue;
             if (elected()) {
 #pragma unroll
                 for (int i = 0; i < kTileTokens / 16; ++i)
                     mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * i, b + i * (2048 >> 4), O_DESC, j > 0 || i > 0);
-                if (j + 1 == steps) commit(bar.o_full(x));
+                if (!more) commit(bar.o_full(x));
             }
             __syncwarp();
-            if (j + 1 < steps) scores(x, (n + 1) & 1);
+            if (more) scores(x, (n + 1) & 1);
         }
         if (ok) {
             release(bar.v_empty(n & 1));
-            if (j + 1 < steps) release(bar.k_empty((n + 1) & 1));
+            if (more) release(bar.k_empty((n + 1) & 1));
         }
     }
 }
@@ -516,35 +546,40 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                 const int rt = threadIdx.x & 127;  // row of the tile = TMEM lane
                 if (x < tiles) {
                     if (steps > 0) {
-                        // Q: one row per warp and turn, scaled by a power of two to f16
-#pragma unroll 2
-                        for (int i = 0; i < 32; ++i) {
-                            const int r = 32 * (w & 3) + i, col = W.col0 + kTileRows * x + r;
-                            constexpr int N = D / 32;
-                            float y[N];
-                            uint32_t mx = 0;
-                            if (col < W.cols) {
-                                const int t = col / A.group;
-                                load_row<N>(A.q, (size_t)(sq.a + t) * A.qs + ((size_t)W.h * A.group + (col - t * A.group)) * D + lane * N,
-                                            A.type, y);
-                            }
+                        // Q: each thread its row, scaled by a power of two to f16
+                        const int t = (W.col0 + kTileRows * x + rt) / A.group, hq = W.col0 + kTileRows * x + rt - t * A.group;
+                        const bool there = W.col0 + kTileRows * x + rt < W.cols;
+                        const uint4 *from = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(A.q) +
+                                                                            (size_t)(sq.a + t) * A.qs +
+                                                                            ((size_t)W.h * A.group + hq) * D);
+                        uint4 y[D / 8];
 #pragma unroll
-                            for (int z = 0; z < N; ++z) {
-                                if (col >= W.cols) y[z] = 0.0f;
-                                mx = max(mx, __float_as_uint(y[z]) & 0x7fffffffu);
-                            }
-                            mx = __reduce_max_sync(0xffffffffu, mx);
-                            int e = 140 - (int)(mx >> 23);  // the largest |q| to [2^13, 2^14)
-                            e = mx == 0 || mx >= 0x7f800000u ? 0 : max(-100, min(100, e));
-                            const float f = __int_as_float((127 + e) << 23);
-                            uint32_t p[N / 2];
+                        for (int i = 0; i < D / 8; ++i) y[i] = there ? from[i] : make_uint4(0, 0, 0, 0);
+                        uint32_t mx = 0;  // the largest |q|, in its own type's bits
 #pragma unroll
-                            for (int z = 0; z < N / 2; ++z) p[z] = pack_half(y[2 * z] * f, y[2 * z + 1] * f);
-                            uint8_t *to = sm.q[x] + swizzled(r, lane * N / 8) + (lane * N % 8) * 2;
-                            if constexpr (N == 2) *reinterpret_cast<uint32_t *>(to) = p[0];
-                            else *reinterpret_cast<uint2 *>(to) = make_uint2(p[0], p[1]);
-                            if (lane == 0) sm.qscale[x][r] = A.scale * __int_as_float((127 - e) << 23);
+                        for (int i = 0; i < D / 8; ++i) {
+                            const uint32_t u[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) mx = max(mx, max(u[z] & 0x7fffu, u[z] >> 16 & 0x7fffu));
                         }
+                        float f = 1.0f;  // f16 stays as it is
+                        if (A.type == Q4RDNA_BF16) {
+                            int e = 140 - (int)(mx >> 7);  // the largest |q| to [2^13, 2^14)
+                            e = mx == 0 || mx >= 0x7f80u ? 0 : max(-100, min(100, e));
+                            f = __int_as_float((127 + e) << 23);
+#pragma unroll
+                            for (int i = 0; i < D / 8; ++i) {
+                                uint32_t u[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+                                for (int z = 0; z < 4; ++z)
+                                    u[z] = pack_half(__uint_as_float(u[z] << 16) * f, __uint_as_float(u[z] & 0xffff0000u) * f);
+                                y[i] = make_uint4(u[0], u[1], u[2], u[3]);
+                            }
+                            f = __int_as_float((127 - e) << 23);
+                        }
+#pragma unroll
+                        for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4 *>(sm.q[x] + swizzled(rt, i)) = y[i];
+                        sm.qscale[x][rt] = A.scale * f;
                         fence_async();
                         __syncwarp();
                         if (lane == 0) bar_arrive(bar.q_full(x));
