@@ -56,12 +56,11 @@ __device__ __forceinline__ void pairs_of(uint32_t a, uint32_t b, uint32_t (&r)[4
         r[2] = sub_1152(__byte_perm(hi, 0x64646464u, 0x4140));
         r[3] = sub_1152(__byte_perm(hi, 0x64646464u, 0x4342));
     } else {
-        const uint32_t sel[4] = {0x4000, 0x5010, 0x6020, 0x7030};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t p = __byte_perm(a, b, sel[i]);  // bytes 1 and 3; the others are masked off
-            r[i] = ((p >> 1) & 0x3f803f80u) | (p & 0x80008000u);
-        }
+        const uint32_t lo = __byte_perm(a, b, 0x5140), hi = __byte_perm(a, b, 0x7362);
+        r[0] = e4m3_pair<false>(lo);
+        r[1] = e4m3_pair<true>(lo);
+        r[2] = e4m3_pair<false>(hi);
+        r[3] = e4m3_pair<true>(hi);
     }
 }
 
@@ -151,7 +150,7 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
                 }
             }
             if (lane == 0)
-                sm.qscale[j] = A.scale * __int_as_float((127 - e) << 23) * (FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f);
+                sm.qscale[j] = A.scale * __int_as_float((127 - e) << 23);
         }
         __syncthreads();
 
@@ -279,8 +278,16 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
                     if constexpr (TERMS == 2) x[z] += sa[n][1][z];
                     x[z] *= scale.x * cs[n][z & 1];
                 }
-                sv[n][0] = sv[n][1] = scale.y * (FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f);
+                sv[n][0] = sv[n][1] = scale.y;
                 if (!whole) {
+                    if (FMT == Q4RDNA_KV_E4M3 && n == 0) {
+                        // rows of the tile that hold no token yet may hold NaN, which a weight of 0 would keep
+#pragma unroll
+                        for (int t = 0; t < 4; ++t)
+                            if (cur * kBlock + 4 * c + t > last)
+#pragma unroll
+                                for (int i = 0; i < VB / 4; ++i) vr[t][i] = 0;
+                    }
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
                         const int tok = cur * kBlock + t0 + (z & 2);

@@ -318,7 +318,7 @@ struct LoadPlace {
     float4 (*scale)[8];
     uint32_t k_full, k_empty, v_full, v_empty, sc_full;
     uint32_t steps, it;
-    int begin, s, h, lo, hi;                     // first step; sequence, head and its visible 16-token blocks
+    int begin, s, h, lo, hi, len;                // first step; sequence, head, its visible 16-token blocks and length
 };
 
 // K and V of a task's steps, from 8-bit tiles to f16 operands (the loading warps)
@@ -339,13 +339,14 @@ __device__ __noinline__ bool load_steps(const AttnArgs &A, const LoadPlace &plac
         const int blk = step * 8 + (lane & 7);
         mine = blk >= P.lo && blk < P.hi ? (unsigned long long)tile_of(A.c, A.b, P.s, P.h, blk) : 0ull;
     };
-    auto load = [&](uint4(&r)[N], int z) {
+    // (a row that holds no token yet may hold NaN, which a weight of 0 would keep: zeros too)
+    auto load = [&](uint4(&r)[N], int z, int tokens) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int t = tk + i * STEP;
             const uint8_t *p = (const uint8_t *)__shfl_sync(0xffffffffu, mine, t >> 4);
             r[i] = make_uint4(0, 0, 0, 0);
-            if (t < kTileTokens && p != nullptr)
+            if (t < tokens && p != nullptr)
                 r[i] = *reinterpret_cast<const uint4 *>(p + kHeader + (z * kBlock + (t & 15)) * D + 16 * ch);
         }
     };
@@ -372,9 +373,10 @@ __device__ __noinline__ bool load_steps(const AttnArgs &A, const LoadPlace &plac
         fence_async();
         __syncwarp();
     };
+    int tokens = min(kTileTokens, P.len - P.begin * kTileTokens);
     find(P.begin);
-    load(kr, 0);
-    load(vr, 1);
+    load(kr, 0, tokens);
+    load(vr, 1, tokens);
 #pragma unroll 1
     for (uint32_t j = 0; j < P.steps; ++j) {
         const uint32_t n = P.it + j, stage = n & 1, parity = ((n >> 1) & 1) ^ 1;
@@ -384,21 +386,21 @@ __device__ __noinline__ bool load_steps(const AttnArgs &A, const LoadPlace &plac
         if (lane == 0) bar_arrive(P.k_full + 8 * stage);
         if (u < 32) {
             if (u < 8) {
-                constexpr float M = FMT == Q4RDNA_KV_E4M3 ? 256.0f : 1.0f;  // e4m3 numbers come as 2^-8 of theirs
-                const float sv = head.y <= kTinyScale ? kTinyScale : head.y * M;  // NaN stays
-                P.scale[n & 3][u] = make_float4(head.x * M, log2f(sv), 1.0f / sv, 0.0f);
+                const float sv = head.y <= kTinyScale ? kTinyScale : head.y;  // NaN stays
+                P.scale[n & 3][u] = make_float4(head.x, log2f(sv), 1.0f / sv, 0.0f);
             }
             __syncwarp();
             if (lane == 0) bar_arrive(P.sc_full + 8 * (n & 3));
         }
         if (j + 1 < P.steps) {
+            tokens = min(kTileTokens, P.len - (P.begin + (int)j + 1) * kTileTokens);
             find(P.begin + (int)j + 1);
-            load(kr, 0);
+            load(kr, 0, tokens);
         }
         bar_wait(P.v_empty + 8 * stage, parity, ok);
         put(P.v + stage * STAGE, vr);
         if (lane == 0) bar_arrive(P.v_full + 8 * stage);
-        if (j + 1 < P.steps) load(vr, 1);
+        if (j + 1 < P.steps) load(vr, 1, tokens);
     }
     return ok;
 }
@@ -668,6 +670,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                     p.h = W.h;
                     p.lo = sp.lo;
                     p.hi = sp.hi;
+                    p.len = sq.L;
                     ok = load_steps<D, FMT>(A, p, ok);
                 }
             } else {
