@@ -4,6 +4,7 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <set>
@@ -186,6 +187,11 @@ Variant variant(int format, int nt, int terms) {
     return format == Q4RDNA_KV_INT8 ? variant<D, Q4RDNA_KV_INT8>(nt, terms) : variant<D, Q4RDNA_KV_E4M3>(nt, terms);
 }
 template <int D>
+Variant tile32_variant(int format) {
+    return {format == Q4RDNA_KV_INT8 ? kv_tile32_kernel<D, Q4RDNA_KV_INT8> : kv_tile32_kernel<D, Q4RDNA_KV_E4M3>,
+            sizeof(TileSmem<D>), kTileThreads, kTile32Cols, kTileShift};
+}
+template <int D>
 Variant tile_variant(int format) {
     return {format == Q4RDNA_KV_INT8 ? kv_tile_kernel<D, Q4RDNA_KV_INT8> : kv_tile_kernel<D, Q4RDNA_KV_E4M3>,
             sizeof(TileSmem<D>), kTileThreads, kTileCols, kTileShift};
@@ -232,14 +238,17 @@ q4rdna_status size_launch(const AttnArgs &A, int D, AttnLaunch &L) {
     return Q4RDNA_OK;
 }
 
-// Columns from which on the tile kernel takes a sequence
-constexpr int kTileFrom = 48;
+// Columns from which on the tile kernels take a sequence
+const int kTileFrom = getenv("TF") ? atoi(getenv("TF")) : 48;
+const int kTile32From = getenv("TF32") ? atoi(getenv("TF32")) : 48;
 
 // The launches of a call: sequences of few columns, sequences of many, or both
 q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &n) {
     n = 0;
     const long long most = A.b.q_start == nullptr ? A.group : (long long)A.b.T * A.group;  // columns of a sequence
-    const bool tiles = D <= 128 && A.type != Q4RDNA_F32 && most >= kTileFrom;
+    const bool f32 = A.type == Q4RDNA_F32;
+    const int from = f32 ? kTile32From : kTileFrom;
+    const bool tiles = D <= 128 && most >= from;
     if (!tiles || (A.b.S > 1 && A.b.q_start != nullptr)) {
         // one column tile where a token's heads fit it and each sequence has one token, else two
         const int nt = A.b.q_start == nullptr && A.group <= 8 ? 1 : 2, terms = A.type == Q4RDNA_F32 ? 2 : 1;
@@ -247,13 +256,14 @@ q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &
         l.v = D == 64 ? variant<64>(A.c.format, nt, terms)
                       : D == 128 ? variant<128>(A.c.format, nt, terms) : variant<256>(A.c.format, nt, terms);
         l.few = 0;
-        l.many = tiles ? kTileFrom : INT_MAX;
+        l.many = tiles ? from : INT_MAX;
         l.min_share = kAttnWarps;  // one block per warp
     }
     if (tiles) {
         AttnLaunch &l = L[n++];
-        l.v = D == 64 ? tile_variant<64>(A.c.format) : tile_variant<128>(A.c.format);
-        l.few = n == 2 ? kTileFrom : 0;
+        if (f32) l.v = D == 64 ? tile32_variant<64>(A.c.format) : tile32_variant<128>(A.c.format);
+        else l.v = D == 64 ? tile_variant<64>(A.c.format) : tile_variant<128>(A.c.format);
+        l.few = n == 2 ? from : 0;
         l.many = INT_MAX;
         l.min_share = 2;
     }

@@ -36,6 +36,7 @@ constexpr int kTileWarps = 16, kTileLoadWarps = 7, kTileMmaWarp = 15;
 constexpr int kTileThreads = 32 * kTileWarps;
 constexpr int kTileRows = 128, kTileTokens = 128, kTileCols = 256, kTileShift = 7;
 constexpr int kTileLoaders = 32 * kTileLoadWarps;
+constexpr int kTileAhead = 7;  // pieces of a loading thread in flight: what shared memory holds
 constexpr unsigned kFaultTile = 16u;
 constexpr uint64_t kTileWaitNs = 1000000000ull;
 
@@ -46,12 +47,16 @@ struct TileSmem {
     uint8_t q[2][STAGE];
     uint8_t k[2][STAGE];
     uint8_t v[2][STAGE];
+    uint8_t ring[kTileAhead * kTileLoaders * 16];  // pieces of the loading threads on their way
     float4 scale[4][8];  // per block of a step: key scale, log2 and inverse of the value scale
     float qscale[2][kTileRows];
-    uint64_t bar[24];
+    float turn[4][kTileRows], sum[kTileRows * 4], ref[kTileRows * 4];  // f32 rows: O's factor, sum and reference (rings of 4 steps)
+    uint64_t bar[28];
     ShareSmem<kTileWarps> share;
     uint32_t tmem;
 };
+
+static_assert(sizeof(TileSmem<128>) <= 232448, "shared memory of the tile kernels");
 
 // ------------------------------------------------------------ PTX
 
@@ -315,93 +320,117 @@ __device__ __noinline__ bool softmax_rows(RowState &row, const RowPlace &at, con
 
 struct LoadPlace {
     uint8_t *k, *v;                              // two stages each
+    uint8_t *ring;
     float4 (*scale)[8];
     uint32_t k_full, k_empty, v_full, v_empty, sc_full;
     uint32_t steps, it;
     int begin, s, h, lo, hi, len;                // first step; sequence, head, its visible 16-token blocks and length
 };
 
-// K and V of a task's steps, from 8-bit tiles to f16 operands (the loading warps)
+// K and V of a task's steps, from 8-bit tiles to f16 operands (the loading warps).  A
+// thread's pieces are 16 codes of a token, N of K and then N of V in every step; they
+// come through a ring of its own in shared memory, kTileAhead pieces ahead (HBM takes
+// about 1500 cycles to answer, a step's conversion 2500).  8 lanes of a store are 4
+// pieces of 2 tokens: all banks once.
 template <int D, int FMT>
 __device__ __noinline__ bool load_steps(const AttnArgs &A, const LoadPlace &place, bool ok) {
     const LoadPlace P = place;
     const int u = threadIdx.x - 32 * (kTileMmaWarp - kTileLoadWarps), lane = threadIdx.x & 31;
-    constexpr int PIECES = D / 16;                      // 16 codes each, of a token
-    constexpr int STEP = kTileLoaders / PIECES;         // tokens from piece to piece of a thread
+    constexpr int PIECES = D / 16;
+    constexpr int STEP = kTileLoaders / PIECES;         // tokens from piece to piece of a thread: 28 or 56
     constexpr int N = (kTileTokens + STEP - 1) / STEP;  // pieces of a thread, K or V of a step
     constexpr int STAGE = TileSmem<D>::STAGE;
-    const int ch = u % PIECES, tk = u / PIECES;
-    const uint32_t odd = (ch >> 2) & 1;
-    uint4 kr[N], vr[N];
-    unsigned long long mine = 0;  // lane i < 8: the tile of block i of the step to be read, or 0: zeros
-    float2 head = make_float2(0.0f, 0.0f);
-    auto find = [&](int step) {
-        const int blk = step * 8 + (lane & 7);
-        mine = blk >= P.lo && blk < P.hi ? (unsigned long long)tile_of(A.c, A.b, P.s, P.h, blk) : 0ull;
+    constexpr int SLOT = kTileLoaders * 16;
+    const int ch = D == 128 ? (lane & 3) | (lane >> 1 & 4) : lane & 3;
+    const int tk = D == 128 ? 4 * (u >> 5) + (lane >> 2 & 1) + (lane >> 3 & 2) : u >> 2;
+    const uint32_t to = swizzled(tk, 2 * ch);
+    const uint32_t from = kHeader + (tk & 3) * D + 16 * ch;
+    const uint32_t ring = smem_u32(P.ring) + 16 * u;
+    const uint8_t *const ring_at = P.ring + 16 * u;
+    // lane i < 8: the tile of block i of steps j, j + 1 and j + 2, or 0: zeros
+    unsigned long long tile0 = 0, tile1 = 0, tile2 = 0;
+    auto find = [&](int j) -> unsigned long long {
+        const int blk = (P.begin + j) * 8 + (lane & 7);
+        return j < (int)P.steps && blk >= P.lo && blk < P.hi ? (unsigned long long)tile_of(A.c, A.b, P.s, P.h, blk) : 0ull;
     };
-    // (a row that holds no token yet may hold NaN, which a weight of 0 would keep: zeros too)
-    auto load = [&](uint4(&r)[N], int z, int tokens) {
+    // Piece i of half z of step j + ahead.  A row that holds no token yet may hold NaN, which
+    // a weight of 0 would keep: zeros there, too.
+    int put_slot = 0, get_slot = 0;
+    auto issue = [&](int j, int ahead, int z, int i) {
+        const int t = tk + i * STEP;
+        const unsigned long long p =
+            __shfl_sync(0xffffffffu, ahead == 0 ? tile0 : ahead == 1 ? tile1 : tile2, (t >> 4) & 7);
+        const bool there = p != 0 && t + (P.begin + j + ahead) * kTileTokens < P.len && (i + 1 < N || t < kTileTokens);
+        const unsigned long long src =
+            there ? p + from + (z * kBlock + (t & 15) - (tk & 3)) * D : (unsigned long long)A.c.tiles;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ring + put_slot), "l"(src), "r"(there ? 16 : 0)
+                     : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        put_slot = put_slot == (kTileAhead - 1) * SLOT ? 0 : put_slot + SLOT;
+    };
+    auto take = [&]() -> uint4 {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kTileAhead - 2) : "memory");
+        const uint4 r = *reinterpret_cast<const uint4 *>(ring_at + get_slot);
+        get_slot = get_slot == (kTileAhead - 1) * SLOT ? 0 : get_slot + SLOT;
+        return r;
+    };
+    auto put = [&](uint8_t *stage, int i, const uint4 &r) {
+        const uint32_t wd[4] = {r.x, r.y, r.z, r.w};
+        uint32_t h[8];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int t = tk + i * STEP;
-            const uint8_t *p = (const uint8_t *)__shfl_sync(0xffffffffu, mine, t >> 4);
-            r[i] = make_uint4(0, 0, 0, 0);
-            if (t < tokens && p != nullptr)
-                r[i] = *reinterpret_cast<const uint4 *>(p + kHeader + (z * kBlock + (t & 15)) * D + 16 * ch);
+        for (int z = 0; z < 4; ++z) {
+            const uint32_t y = FMT == Q4RDNA_KV_INT8 ? wd[z] ^ 0x80808080u : wd[z];
+            h[2 * z] = pair_of<FMT, 0>(y);
+            h[2 * z + 1] = pair_of<FMT, 2>(y);
+        }
+        if (i + 1 < N || tk + i * STEP < kTileTokens) {
+            // the swizzle of token tk + i STEP: STEP is a multiple of 4
+            const uint32_t at = (to ^ ((i * STEP & 4) << 4)) + i * STEP * 128;
+            *reinterpret_cast<uint4 *>(stage + at) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4 *>(stage + (at ^ 16)) = make_uint4(h[4], h[5], h[6], h[7]);
         }
     };
-    auto put = [&](uint8_t *stage, const uint4(&r)[N]) {
+    tile0 = find(0);
+    tile1 = find(1);
+    float2 head = u < 8 && tile0 != 0 ? *reinterpret_cast<const float2 *>(tile0) : make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int t = tk + i * STEP;
-            if (t >= kTileTokens) break;
-            const uint32_t wd[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-            uint32_t h[8];
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const uint32_t y = FMT == Q4RDNA_KV_INT8 ? wd[z] ^ 0x80808080u : wd[z];
-                h[2 * z] = pair_of<FMT, 0>(y);
-                h[2 * z + 1] = pair_of<FMT, 2>(y);
-            }
-            // the two halves in an order that keeps a phase's lanes in different banks
-            uint8_t *const to = stage + swizzled(t, 2 * ch + odd);
-            uint8_t *const too = stage + swizzled(t, 2 * ch + (odd ^ 1));
-            const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
-            *reinterpret_cast<uint4 *>(to) = odd ? b : a;
-            *reinterpret_cast<uint4 *>(too) = odd ? a : b;
-        }
-        fence_async();
-        __syncwarp();
-    };
-    int tokens = min(kTileTokens, P.len - P.begin * kTileTokens);
-    find(P.begin);
-    load(kr, 0, tokens);
-    load(vr, 1, tokens);
+    for (int a = 0; a < kTileAhead; ++a) issue(0, a / (2 * N), a / N % 2, a % N);
 #pragma unroll 1
     for (uint32_t j = 0; j < P.steps; ++j) {
         const uint32_t n = P.it + j, stage = n & 1, parity = ((n >> 1) & 1) ^ 1;
-        if (u < 8) head = mine != 0 ? *reinterpret_cast<const float2 *>(mine) : make_float2(0.0f, 0.0f);
-        bar_wait(P.k_empty + 8 * stage, parity, ok);
-        put(P.k + stage * STAGE, kr);
-        if (lane == 0) bar_arrive(P.k_full + 8 * stage);
-        if (u < 32) {
-            if (u < 8) {
-                const float sv = head.y <= kTinyScale ? kTinyScale : head.y;  // NaN stays
-                P.scale[n & 3][u] = make_float4(head.x, log2f(sv), 1.0f / sv, 0.0f);
+        tile2 = find(j + 2);
+        const float2 next_head = u < 8 && tile1 != 0 ? *reinterpret_cast<const float2 *>(tile1) : make_float2(0.0f, 0.0f);
+        uint4 r = take();
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            bar_wait((z == 0 ? P.k_empty : P.v_empty) + 8 * stage, parity, ok);
+            uint8_t *const to_stage = (z == 0 ? P.k : P.v) + stage * STAGE;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                constexpr int A0 = kTileAhead;
+                const int a = z * N + i + A0;
+                const uint4 now = r;
+                if (z == 0 || i + 1 < N) r = take();
+                put(to_stage, i, now);
+                issue(j, a / (2 * N), a / N % 2, a % N);  // into the slot that `now` came from
             }
+            fence_async();
             __syncwarp();
-            if (lane == 0) bar_arrive(P.sc_full + 8 * (n & 3));
+            if (lane == 0) bar_arrive((z == 0 ? P.k_full : P.v_full) + 8 * stage);
+            if (z == 0 && u < 32) {
+                if (u < 8) {
+                    const float sv = head.y <= kTinyScale ? kTinyScale : head.y;  // NaN stays
+                    P.scale[n & 3][u] = make_float4(head.x, log2f(sv), 1.0f / sv, 0.0f);
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(P.sc_full + 8 * (n & 3));
+            }
         }
-        if (j + 1 < P.steps) {
-            tokens = min(kTileTokens, P.len - (P.begin + (int)j + 1) * kTileTokens);
-            find(P.begin + (int)j + 1);
-            load(kr, 0, tokens);
-        }
-        bar_wait(P.v_empty + 8 * stage, parity, ok);
-        put(P.v + stage * STAGE, vr);
-        if (lane == 0) bar_arrive(P.v_full + 8 * stage);
-        if (j + 1 < P.steps) load(vr, 1, tokens);
+        tile0 = tile1;
+        tile1 = tile2;
+        head = next_head;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     return ok;
 }
 
@@ -427,7 +456,83 @@ struct Bars {
     __device__ __forceinline__ uint32_t p_full(int x) const { return at + 8u * (16 + x); }
     __device__ __forceinline__ uint32_t o_full(int x) const { return at + 8u * (18 + x); }
     __device__ __forceinline__ uint32_t drained() const { return at + 8u * 20; }
+    // f32 rows: the step's O read, and O's factor written (ring of 4)
+    __device__ __forceinline__ uint32_t o_free() const { return at + 8u * 21; }
+    __device__ __forceinline__ uint32_t turned(int i) const { return at + 8u * (22 + i); }
 };
+
+// Tensor memory and barriers at the kernel's begin and end
+template <int D>
+__device__ __forceinline__ uint32_t tile_enter(TileSmem<D> &sm, Bars bar) {
+    if ((threadIdx.x >> 5) == kTileMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            bar_init(bar.k_full(i), kTileLoadWarps);
+            bar_init(bar.v_full(i), kTileLoadWarps);
+            bar_init(bar.k_empty(i), 1);
+            bar_init(bar.v_empty(i), 1);
+            bar_init(bar.q_full(i), 4);
+            bar_init(bar.s_full(i), 1);
+            bar_init(bar.p_full(i), 4);
+            bar_init(bar.o_full(i), 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            bar_init(bar.sc_full(i), 1);
+            bar_init(bar.turned(i), 4);
+        }
+        bar_init(bar.o_free(), 4);
+        bar_init(bar.drained(), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    return sm.tmem;
+}
+__device__ __forceinline__ void tile_leave(uint32_t tmem, Bars bar) {
+    const bool mine = (threadIdx.x >> 5) == kTileMmaWarp;
+    if (mine) {  // no product may still run when the tensor memory goes
+        bool last = true;
+        if (elected()) commit(bar.drained());
+        __syncwarp();
+        bar_wait(bar.drained(), 0, last);
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (mine) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// The loading warps' part of a task
+template <int D, int FMT>
+__device__ __forceinline__ bool load_task(const AttnArgs &A, TileSmem<D> &sm, Bars bar, const Walk &W, int nc, int steps,
+                                          uint32_t it, bool ok) {
+    // 16-token blocks that a column of the task sees
+    const Span sp = span_of(W.q, W.col0, nc, A.group, A.window, 4);
+    LoadPlace p;
+    p.k = sm.k[0];
+    p.v = sm.v[0];
+    p.ring = sm.ring;
+    p.scale = sm.scale;
+    p.k_full = bar.k_full(0);
+    p.k_empty = bar.k_empty(0);
+    p.v_full = bar.v_full(0);
+    p.v_empty = bar.v_empty(0);
+    p.sc_full = bar.sc_full(0);
+    p.steps = steps;
+    p.it = it;
+    p.begin = W.begin;
+    p.s = W.s;
+    p.h = W.h;
+    p.lo = sp.lo;
+    p.hi = sp.hi;
+    p.len = W.q.L;
+    return load_steps<D, FMT>(A, p, ok);
+}
 
 // The products of a task's steps.  Order: S0 S1 of the first step, then per step and
 // tile O += P V and the next step's S.  st, tt: steps and tasks of either tile so far.
@@ -504,30 +609,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
     const Bars bar{smem_u32(sm.bar)};
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (w == kTileMmaWarp) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
-            bar_init(bar.k_full(i), kTileLoadWarps);
-            bar_init(bar.v_full(i), kTileLoadWarps);
-            bar_init(bar.k_empty(i), 1);
-            bar_init(bar.v_empty(i), 1);
-            bar_init(bar.q_full(i), 4);
-            bar_init(bar.s_full(i), 1);
-            bar_init(bar.p_full(i), 4);
-            bar_init(bar.o_full(i), 1);
-        }
-        for (int i = 0; i < 4; ++i) bar_init(bar.sc_full(i), 1);
-        bar_init(bar.drained(), 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    fence_before();
-    __syncthreads();
-    fence_after();
-    const uint32_t tmem = sm.tmem;
+    const uint32_t tmem = tile_enter<D>(sm, bar);
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const long long left = find_share<kTileWarps>(A, kTileCols, kTileShift, sm.share);
@@ -652,26 +734,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
             } else if (w < kTileMmaWarp) {
                 // ------------------------------------------------ loading
                 if (steps > 0) {
-                    // 16-token blocks that a column of the task sees
-                    const Span sp = span_of(sq, W.col0, kTileCols, A.group, A.window, 4);
-                    LoadPlace p;
-                    p.k = sm.k[0];
-                    p.v = sm.v[0];
-                    p.scale = sm.scale;
-                    p.k_full = bar.k_full(0);
-                    p.k_empty = bar.k_empty(0);
-                    p.v_full = bar.v_full(0);
-                    p.v_empty = bar.v_empty(0);
-                    p.sc_full = bar.sc_full(0);
-                    p.steps = steps;
-                    p.it = it;
-                    p.begin = W.begin;
-                    p.s = W.s;
-                    p.h = W.h;
-                    p.lo = sp.lo;
-                    p.hi = sp.hi;
-                    p.len = sq.L;
-                    ok = load_steps<D, FMT>(A, p, ok);
+                    ok = load_task<D, FMT>(A, sm, bar, W, kTileCols, steps, it, ok);
                 }
             } else {
                 // ------------------------------------------------ products
@@ -693,18 +756,323 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
         }
     }
     if (threadIdx.x == 0 && !open) A.rec[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (w == kTileMmaWarp) {  // no product may still run when the tensor memory goes
-        bool last = true;
-        if (elected()) commit(bar.drained());
+    tile_leave(tmem, bar);
+}
+
+// ------------------------------------------------------------ f32 rows
+//
+// The same for f32 rows, in the same precision as the kernel for few columns: q and p as
+// two f16 terms each (22 bits), and O summed in f32 by a warpgroup of its own, because
+// the tensor core's running sum truncates (measured: 1 + 1.9 * 2^-24 stays 1), which over
+// a task's products would cost 2^-17.  A task is 128 columns, one tile; Q's two terms
+// take the two Q buffers, S two buffers in turn (the next step's S is made under this
+// step's softmax), then the step's O and the task's O.  Warps 4-7 add one to the other.
+
+constexpr int kTile32Cols = 128;
+
+// Columns 32 c .. of S become the step's weights: 16 columns of first terms, 16 of second ones
+template <int D>
+__device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm, Bars bar, uint32_t tmem, int steps,
+                                            uint32_t it, int tok0, bool ok) {
+    RowState r = row;
+    const int rt = threadIdx.x;
+    const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
+    const int all_lo = __reduce_max_sync(0xffffffffu, r.lo), all_hi = __reduce_min_sync(0xffffffffu, r.hi);
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j, tok0 += kTileTokens) {
+        const uint32_t n = it + j;
+        bar_wait(bar.s_full(n & 1), (n >> 1) & 1, ok);
+        bar_wait(bar.sc_full(n & 3), (n >> 2) & 1, ok);  // at most one phase ahead once S is there
+        fence_after();
+        const uint32_t s_at = tmem + lanes + 128 * (n & 1);
+        const float4 *const scale = sm.scale[n & 3];
+        uint32_t v[32];
+        auto hide = [&](int tok) {
+            if (tok < all_lo || tok + 31 > all_hi) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (tok + i < r.lo || tok + i > r.hi) v[i] = 0xff800000u;  // -inf
+            }
+        };
+        float t = -INFINITY;  // the largest exponent
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+            tmem_load32(s_at + 32 * c, v);
+            tmem_wait_load();
+            hide(tok0 + 32 * c);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float4 f = scale[2 * c + b];
+                float m = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, __uint_as_float(v[16 * b + i]));
+                // a block without a visible token has m = -inf, which a scale of 0 would turn into NaN
+                if (m != -INFINITY) t = fmaxf(t, fmaf(m, f.x * r.scale, f.y));
+            }
+        }
+        float f = 1.0f;
+        if (t > r.R + 8.0f) {  // also the first: R = -inf
+            f = ex2(r.R - t);
+            r.R = t;
+            r.l *= f;
+        }
+        const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+            uint32_t p[32];
+            tmem_load32(s_at + 32 * c, v);
+            tmem_wait_load();
+            const int tok = tok0 + 32 * c;
+            const bool part = tok < all_lo || tok + 31 > all_hi;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float4 g = scale[2 * c + b];
+                const float a = g.x * r.scale, d = g.y - ref;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    float e[2];
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        float x = fmaf(__uint_as_float(v[16 * b + i + z]), a, d);
+                        const int at = tok + 16 * b + i + z;
+                        if (part && (at < r.lo || at > r.hi)) x = -INFINITY;
+                        e[z] = ex2(x);
+                    }
+                    sum += e[0] + e[1];
+                    const uint32_t hi = pack_half(e[0], e[1]);
+                    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                    p[8 * b + i / 2] = hi;
+                    p[16 + 8 * b + i / 2] = pack_half(e[0] - h.x, e[1] - h.y);
+                }
+                // a block without a visible token takes nothing from its scale, be it NaN
+                if (sum != 0.0f) r.l = fmaf(sum, g.z, r.l);
+            }
+            tmem_store32(s_at + 32 * c, p);
+        }
+        tmem_wait_store();
+        fence_before();
+        sm.turn[n & 3][rt] = f;
+        if (j + 1 == steps) {
+            sm.sum[128 * (n & 3) + rt] = r.l;
+            sm.ref[128 * (n & 3) + rt] = r.R;
+        }
         __syncwarp();
-        bar_wait(bar.drained(), 0, last);
+        if ((threadIdx.x & 31) == 0) {
+            bar_arrive(bar.p_full(0));
+            bar_arrive(bar.turned(n & 3));
+        }
     }
-    fence_before();
-    __syncthreads();
+    return ok;
+}
+
+// O = O * f + the step's O; after the last step to the output
+template <int D>
+__device__ __noinline__ bool add32_rows(const AttnArgs &A, const Walk &W, TileSmem<D> &sm, Bars bar, uint32_t tmem, int steps,
+                                        uint32_t it, bool ok) {
+    const int rt = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
+    const uint32_t step_at = tmem + lanes + 256, o_at = tmem + lanes + 384;
+    const bool whole = W.whole();
+    const int col = W.col0 + rt;
+    const bool there = col < W.cols;
+    const int tok = there ? col / A.group : 0;
+    float *const part = W.part(D);
+    const size_t at = (size_t)(W.q.a + tok) * A.os + ((size_t)W.h * A.group + (there ? col - tok * A.group : 0)) * D;
+    for (int j = 0; j < max(steps, 1); ++j) {
+        const uint32_t n = it + j;
+        float f = 1.0f, l = 0.0f, R = -INFINITY;
+        const bool last = j + 1 >= steps;
+        if (steps > 0) {
+            bar_wait(bar.o_full(0), n & 1, ok);
+            bar_wait(bar.turned(n & 3), (n >> 2) & 1, ok);  // at most one phase ahead once the step's O is there
+            fence_after();
+            f = sm.turn[n & 3][rt];
+            if (last) {
+                l = sm.sum[128 * (n & 3) + rt];
+                R = sm.ref[128 * (n & 3) + rt];
+            }
+        }
+        const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t v[32], u[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = u[i] = 0;
+            if (steps > 0) {
+                tmem_load32(step_at + c, v);
+                if (j > 0) tmem_load32(o_at + c, u);
+                tmem_wait_load();
+            }
+            if (j > 0) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    v[i] = __float_as_uint(fmaf(__uint_as_float(u[i]), f, __uint_as_float(v[i])));
+            }
+            if (!last) {
+                tmem_store32(o_at + c, v);
+            } else if (there) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int z = 0; z < 8; ++z) y[z] = __uint_as_float(v[i + z]) * inv;
+                    if (whole) store_row<8>(A.out, at + c + i, A.type, y);
+                    else store_row<8>(part, (size_t)rt * D + c + i, Q4RDNA_F32, y);
+                }
+            }
+        }
+        if (last && there && !whole) {
+            part[kTile32Cols * D + rt] = R;
+            part[kTile32Cols * D + kTile32Cols + rt] = l;
+        }
+        if (steps > 0) {
+            tmem_wait_store();
+            fence_before();
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) bar_arrive(bar.o_free());
+        }
+    }
+    return ok;
+}
+
+template <int D>
+__device__ __forceinline__ void issue32_steps(TileSmem<D> &sm, uint32_t tmem, Bars bar, int steps, uint32_t it, uint32_t task,
+                                              bool &ok) {
+    using Smem = TileSmem<D>;
+    constexpr uint32_t S_DESC = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | (8u << 24);
+    constexpr uint32_t O_DESC = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+    const uint64_t q0 = operand(smem_u32(sm.q[0]), 16), k0 = operand(smem_u32(sm.k[0]), 16);
+    const uint64_t v0 = operand(smem_u32(sm.v[0]), Smem::PANEL);
+    auto scores = [&](uint32_t n) {
+        const uint64_t b = k0 + (n & 1) * (Smem::STAGE >> 4);
+        if (elected()) {
+#pragma unroll
+            for (int x = 1; x >= 0; --x)  // the second, small terms first: their sum's rounding is small too
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint32_t off = ((i >> 2) * Smem::PANEL + (i & 3) * 32) >> 4;
+                    mma_ss(tmem + 128 * (n & 1), q0 + x * (Smem::STAGE >> 4) + off, b + off, S_DESC, x == 0 || i > 0);
+                }
+            commit(bar.s_full(n & 1));
+            commit(bar.k_empty(n & 1));
+        }
+        __syncwarp();
+    };
+    bar_wait(bar.q_full(0), task & 1, ok);
+    bar_wait(bar.k_full(it & 1), (it >> 1) & 1, ok);
     fence_after();
-    if (w == kTileMmaWarp) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (ok) scores(it);
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j) {
+        const uint32_t n = it + j;
+        if (j + 1 < steps) {
+            // S of the next step goes where the step before this one had its P, whose products were issued earlier
+            bar_wait(bar.k_full((n + 1) & 1), ((n + 1) >> 1) & 1, ok);
+            fence_after();
+            if (ok) scores(n + 1);
+        }
+        if (!bar_try3(bar.p_full(0), n & 1, bar.v_full(n & 1), (n >> 1) & 1, bar.o_free(), (n & 1) ^ 1)) {
+            bar_wait(bar.v_full(n & 1), (n >> 1) & 1, ok);
+            bar_wait(bar.o_free(), (n & 1) ^ 1, ok);
+            bar_wait(bar.p_full(0), n & 1, ok);
+        }
+        fence_after();
+        if (!ok) continue;
+        const uint64_t b = v0 + (n & 1) * (Smem::STAGE >> 4);
+        if (elected()) {
+#pragma unroll
+            for (int x = 1; x >= 0; --x)
+#pragma unroll
+                for (int i = 0; i < kTileTokens / 16; ++i)
+                    mma_ts(tmem + 256, tmem + 128 * (n & 1) + 32 * (i >> 1) + 8 * (i & 1) + 16 * x, b + i * (2048 >> 4), O_DESC,
+                           x == 0 || i > 0);
+            commit(bar.o_full(0));
+            commit(bar.v_empty(n & 1));
+        }
+        __syncwarp();
     }
+}
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kTileThreads, 1) kv_tile32_kernel(const __grid_constant__ AttnArgs A) {
+    using Smem = TileSmem<D>;
+    extern __shared__ __align__(1024) uint8_t tile_smem[];
+    Smem &sm = *reinterpret_cast<Smem *>(tile_smem);
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Bars bar{smem_u32(sm.bar)};
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = tile_enter<D>(sm, bar);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const long long left = find_share<kTileWarps>(A, kTile32Cols, kTileShift, sm.share);
+    bool ok = true, open = false;
+    if (left > 0) {
+        Walk W(A, kTile32Cols, kTileShift, left, sm.share.rest, sm.share.share, sm.share.seq);
+        uint32_t it = 0, task = 0;  // steps and tasks with steps so far
+        while (W.next()) {
+            const Seq &sq = W.q;
+            const int steps = max(0, W.end - W.begin);
+            if (w < 4) {
+                if (steps > 0) {
+                    // Q: each thread its row, scaled by a power of two, in two f16 terms
+                    const int rt = threadIdx.x, col = W.col0 + rt, tok = col / A.group;
+                    const bool there = col < W.cols;
+                    const float4 *from = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(A.q) +
+                                                                          (size_t)(sq.a + (there ? tok : 0)) * A.qs +
+                                                                          ((size_t)W.h * A.group + (there ? col - tok * A.group : 0)) * D);
+                    uint32_t mx = 0;
+#pragma unroll 8
+                    for (int i = 0; i < D / 4; ++i) {
+                        const float4 y = from[i];
+                        mx = max(max(mx, max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu)),
+                                 max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
+                    }
+                    int e = 140 - (int)(mx >> 23);  // the largest |q| to [2^13, 2^14)
+                    e = mx == 0 || mx >= 0x7f800000u ? 0 : max(-100, min(100, e));
+                    const float f = there ? __int_as_float((127 + e) << 23) : 0.0f;
+#pragma unroll 4
+                    for (int i = 0; i < D / 8; ++i) {
+                        const float4 a = from[2 * i], b = from[2 * i + 1];
+                        const float y[8] = {a.x * f, a.y * f, a.z * f, a.w * f, b.x * f, b.y * f, b.z * f, b.w * f};
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            hi[z] = pack_half(y[2 * z], y[2 * z + 1]);
+                            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi[z]));
+                            lo[z] = pack_half(y[2 * z] - h.x, y[2 * z + 1] - h.y);
+                        }
+                        *reinterpret_cast<uint4 *>(sm.q[0] + swizzled(rt, i)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(sm.q[1] + swizzled(rt, i)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(bar.q_full(0));
+                    RowState r;
+                    r.R = -INFINITY;
+                    r.l = 0.0f;
+                    r.scale = A.scale * __int_as_float((127 - e) << 23);
+                    r.hi = there ? sq.L - sq.n + tok : INT_MAX;  // (a padded row is computed and never read)
+                    r.lo = there && A.window > 0 ? max(0, r.hi - A.window + 1) : 0;
+                    ok = softmax32_rows<D>(r, sm, bar, tmem, steps, it, W.begin * kTileTokens, ok);
+                }
+            } else if (w < 8) {
+                ok = add32_rows<D>(A, W, sm, bar, tmem, steps, it, ok);
+            } else if (w < kTileMmaWarp) {
+                if (steps > 0) ok = load_task<D, FMT>(A, sm, bar, W, kTile32Cols, steps, it, ok);
+            } else if (steps > 0) {
+                issue32_steps<D>(sm, tmem, bar, steps, it, task, ok);
+            }
+            it += steps;
+            if (steps > 0) ++task;
+            if (W.open()) {
+                open = true;
+                if (threadIdx.x == 0) W.note();
+            }
+        }
+    }
+    if (threadIdx.x == 0 && !open) A.rec[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+    tile_leave(tmem, bar);
 }
 
 }  // namespace q4kv
