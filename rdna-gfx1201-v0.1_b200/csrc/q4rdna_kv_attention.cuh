@@ -111,7 +111,7 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
     }
     bool open = false;  // the share ends inside a task that began in it
     const int t0 = 4 * (g >> 1) + (g & 1);  // K rows g and g + 8 of the fragments: tokens t0 and t0 + 2
-    Walk W(A, NC, 4, left, sm.share.rest, sm.share.share, sm.share.seq);
+    Walk W(A, NC, 4, left, sm.share);
     while (W.next()) {
         const Seq &sq = W.q;
         const int s = W.s, cols = W.cols, h = W.h, col0 = W.col0, b0 = W.begin, b1 = W.end;

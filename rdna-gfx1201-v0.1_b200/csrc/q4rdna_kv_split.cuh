@@ -80,8 +80,9 @@ template <int WARPS>
 struct ShareSmem {
     long long sum[WARPS];
     long long rest;  // offset of the share's begin in sequence `seq`
-    long long share;
+    long long share, head;  // head: the sequence's work per kv head
     int seq;
+    Seq q;
 };
 
 // Where the CTA's share begins: sequence and offset in its work (in sm); returns the
@@ -91,8 +92,9 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
     constexpr int THREADS = 32 * WARPS;
     const Batch &B = A.b;
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Seq q{0, 0, 0};
     auto work = [&](int s) -> long long {
-        Seq q{0, 0, 0};
+        q = Seq{0, 0, 0};
         if (s < B.S) q = load_seq(B, s);
         return head_work(A, q, nc, shift) * A.c.hk;
     };
@@ -113,7 +115,7 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
     if (threadIdx.x == 0) sm.share = share;
     long long before = 0;
     for (int base = 0; base < B.S && before <= begin; base += THREADS) {
-        const long long mine = base == 0 ? first : work(base + threadIdx.x);
+        const long long mine = base == 0 && B.S <= THREADS ? first : work(base + threadIdx.x);  // (and q)
         long long x = mine;  // inclusive prefix
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -131,6 +133,8 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
         if (at >= 0 && at < mine) {
             sm.seq = base + threadIdx.x;
             sm.rest = at;
+            sm.q = q;
+            sm.head = mine / A.c.hk;
         }
         before += all;
         __syncthreads();
@@ -152,9 +156,14 @@ struct Walk {
     int begin = 0, end = 0, all = 0, cnt = 0;
     bool begins = false, ends = false;
 
-    __device__ __forceinline__ Walk(const AttnArgs &a, int nc_, int shift_, long long left_, long long rest_, long long share_,
-                                    int seq)
-        : A(a), nc(nc_), shift(shift_), left(left_), rest(rest_), share(share_), s(seq - 1), h(a.c.hk) {}
+    template <class Smem>
+    __device__ __forceinline__ Walk(const AttnArgs &a, int nc_, int shift_, long long left_, const Smem &sm)
+        : A(a), nc(nc_), shift(shift_), left(left_), rest(sm.rest), share(sm.share), s(sm.seq), q(sm.q) {
+        cols = q.n * A.group;
+        h = (int)(rest / sm.head);
+        rest -= h * sm.head;
+        col0 = -nc;
+    }
 
     __device__ __forceinline__ bool next() {
         if (left <= 0) return false;
@@ -274,24 +283,47 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_c
         return A.part + (size_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * part_floats(D, nc);
     };
     const int n = min(r1.y, (int)gridDim.x - 1) - (int)blockIdx.x + 1;
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, piece(i)[nc * D + j]);
+    // lane i holds the maximum and sum of piece i (of 32 at a time)
+    float m = -INFINITY, l = 0.0f;
+    if (lane < n) {
+        m = piece(lane)[nc * D + j];
+        l = piece(lane)[nc * D + nc + j];
+    }
+    float M = m;
+    for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, piece(i)[nc * D + j]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float x[EPL], L = 0.0f;
 #pragma unroll
     for (int t = 0; t < EPL; ++t) x[t] = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const float *p = piece(i);
-        const float mi = p[nc * D + j];
-        const float f = mi == -INFINITY ? 1.0f : ex2(mi - M);
-        L = fmaf(f, p[nc * D + nc + j], L);
-        float y[EPL];
-        load_row<EPL>(p, (size_t)j * D + lane * EPL, Q4RDNA_F32, y);
+    for (int base = 0; base < n; base += 32) {
+        if (base > 0) {
+            m = -INFINITY;
+            l = 0.0f;
+            if (base + lane < n) {
+                m = piece(base + lane)[nc * D + j];
+                l = piece(base + lane)[nc * D + nc + j];
+            }
+        }
+        const float f = m == -INFINITY ? 1.0f : ex2(m - M);
+        L = fmaf(f, l, L);
+        const int cnt = min(32, n - base);
+        for (int i = 0; i < cnt; i += 8) {  // 8 pieces on their way
+            float y[8][EPL];
 #pragma unroll
-        for (int t = 0; t < EPL; ++t) x[t] = fmaf(f, y[t], x[t]);
+            for (int u = 0; u < 8; ++u)
+                if (i + u < cnt) load_row<EPL>(piece(base + i + u), (size_t)j * D + lane * EPL, Q4RDNA_F32, y[u]);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float fu = __shfl_sync(0xffffffffu, f, (i + u) & 31);
+                if (i + u < cnt)
+#pragma unroll
+                    for (int t = 0; t < EPL; ++t) x[t] = fmaf(fu, y[u][t], x[t]);
+            }
+        }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     const float r = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
     for (int t = 0; t < EPL; ++t) x[t] *= r;

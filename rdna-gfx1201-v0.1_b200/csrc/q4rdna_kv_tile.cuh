@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
     const long long left = find_share<kTileWarps>(A, kTileCols, kTileShift, sm.share);
     bool ok = true, open = false;
     if (left > 0) {
-        Walk W(A, kTileCols, kTileShift, left, sm.share.rest, sm.share.share, sm.share.seq);
+        Walk W(A, kTileCols, kTileShift, left, sm.share);
         uint32_t it = 0;   // steps so far: stage it % 2
         uint32_t st[2] = {0, 0}, tt[2] = {0, 0};  // steps of either tile, and tasks with steps
         while (W.next()) {
@@ -1008,7 +1008,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile32_kernel(const __grid
     const long long left = find_share<kTileWarps>(A, kTile32Cols, kTileShift, sm.share);
     bool ok = true, open = false;
     if (left > 0) {
-        Walk W(A, kTile32Cols, kTileShift, left, sm.share.rest, sm.share.share, sm.share.seq);
+        Walk W(A, kTile32Cols, kTileShift, left, sm.share);
         uint32_t it = 0, task = 0;  // steps and tasks with steps so far
         while (W.next()) {
             const Seq &sq = W.q;
