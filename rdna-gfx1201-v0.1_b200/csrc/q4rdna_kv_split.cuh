@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_c
     const int4 r1 = A.rec[2 * blockIdx.x + 1];
     const int j = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int col = r0.w + j;
-    if (col >= r0.z) return;
+    if (j >= nc || col >= r0.z) return;
     // piece 0: this CTA's second slot; then the first slots of the CTAs up to the task's last
     auto piece = [&](int i) {
         return A.part + (size_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * part_floats(D, nc);

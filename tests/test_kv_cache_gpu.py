@@ -206,7 +206,8 @@ def test_bad_metadata_sets_the_fault(cuda):
     cache, tiles, table = make(cuda, 880, [40, 40], H, D, P, KV_INT8)
     q = torch.randn((2, H * G, D), device=cuda)
     k = torch.randn((2, H, D), device=cuda)
-    good = q4rdna.kv_attention(cache, KVBatch(table.to(cuda), i32([40, 40], cuda)), q)
+    good = {n: q4rdna.kv_attention(cache, KVBatch(table.to(cuda), i32([40, 40], cuda), q_start=start), q)
+            for n, start in ((False, None), (True, i32([0, 1, 2], cuda)))}  # a kernel each
     assert q4rdna.take_fault() == 0
     bad = table.clone()
     bad[1, 1] = tiles.shape[0]
@@ -214,7 +215,7 @@ def test_bad_metadata_sets_the_fault(cuda):
                               (table, [40, 40], [0, 1, 3]), (table, [40, 40], [0, 1, 0])]:
         batch = KVBatch(t.to(cuda), i32(lengths, cuda), q_start=None if start is None else i32(start, cuda))
         out = q4rdna.kv_attention(cache, batch, q)
-        assert torch.equal(out[0], good[0])
+        assert torch.equal(out[0], good[start is not None][0])
         assert q4rdna.take_fault() == 8
     # the append with the same tables: the other sequence's row is written, nothing else
     for t, lengths in [(bad.roll(0), [33, 17]), (table, [33, 49])]:
