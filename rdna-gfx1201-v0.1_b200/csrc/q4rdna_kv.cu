@@ -397,7 +397,6 @@ q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_
     if (workspace == nullptr || workspace_bytes < bytes) return Q4RDNA_ERR_WORKSPACE;
     if (!aligned(workspace)) return Q4RDNA_ERR_ALIGNMENT;
     const cudaStream_t cs = (cudaStream_t)stream;
-    const auto join = D == 64 ? kv_join_kernel<64> : D == 128 ? kv_join_kernel<128> : kv_join_kernel<256>;
     uint8_t *at = reinterpret_cast<uint8_t *>(workspace);
     for (int i = 0; i < n; ++i) {
         const AttnLaunch &l = L[i];
@@ -408,7 +407,11 @@ q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_
         A.part = reinterpret_cast<float *>(A.rec + 2 * l.grid);
         at += l.workspace;
         if ((st = launch(l.v.kernel, dim3(l.grid), l.v.threads, l.v.smem, cs, A)) != Q4RDNA_OK) return st;
-        if ((st = launch(join, dim3(l.grid, (unsigned)((l.v.nc + kJoinWarps - 1) / kJoinWarps)), 32 * kJoinWarps, 0, cs, A,
+        const bool wide = l.v.nc > 16;
+        const auto join = D == 64    ? (wide ? kv_join_kernel<64, true> : kv_join_kernel<64, false>)
+                          : D == 128 ? (wide ? kv_join_kernel<128, true> : kv_join_kernel<128, false>)
+                                     : (wide ? kv_join_kernel<256, true> : kv_join_kernel<256, false>);
+        if ((st = launch(join, dim3(l.grid, (unsigned)(wide ? l.v.nc / kJoinWarps : l.v.nc)), 32 * kJoinWarps, 0, cs, A,
                          l.v.nc)) != Q4RDNA_OK)
             return st;
     }

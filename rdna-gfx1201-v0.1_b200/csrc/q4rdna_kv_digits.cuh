@@ -105,8 +105,34 @@ __global__ void __launch_bounds__(kDigThreads, 2) kv_digits_kernel(const __grid_
         const int s = W.s, cols = W.cols, h = W.h, col0 = W.col0, b0 = W.begin, b1 = W.end;
         const int first = sq.L - sq.n;  // token of the sequence's first row
 
-        // ---- the ring: this warp's pairs of blocks p, p + 1, then 2 kDigWarps further
-        auto tile_at = [&](int blk) -> const uint8_t * { return blk < b1 ? tile_of(A.c, B, s, h, blk) : nullptr; };
+        // ---- q of this warp's column and the pages of its first 16 pairs, on their way together
+        constexpr int N = D / 32;
+        float qx[N];
+#pragma unroll
+        for (int t = 0; t < N; ++t) qx[t] = 0.0f;
+        if (w < NC && col0 + w < cols) {
+            const int i = (col0 + w) / A.group;
+            load_row<N>(A.q, (size_t)(sq.a + i) * A.qs + ((size_t)h * A.group + (col0 + w - i * A.group)) * D + lane * N, A.type, qx);
+        }
+        // this warp's pairs are blocks p, p + 1, then 2 kDigWarps further; lane i: the page of the
+        // pair i / 2 of 16
+        int p = b0 + 2 * w;
+        auto pages_from = [&](int at) {
+            const int blk = at + 2 * kDigWarps * (lane >> 1) + (lane & 1);
+            return blk < b1 ? B.table[(size_t)s * B.stride + (blk >> A.c.nbl)] : -2;
+        };
+        int pages = pages_from(p);
+        // tile of block blk, the k-th of the 32 that `pages` covers; null: nothing there to read
+        auto tile_at = [&](int blk, int k) -> const uint8_t * {
+            const int page = __shfl_sync(0xffffffffu, pages, k);
+            if ((unsigned)page >= (unsigned)A.c.pages) {
+                if (blk < b1 && lane == 0) atomicOr(&g_kv_fault, kFaultBatch);
+                return nullptr;
+            }
+            const size_t t = (((size_t)page * A.c.hk + h) << A.c.nbl) + (blk & ((1 << A.c.nbl) - 1));
+            return A.c.tiles + t * A.c.tile_bytes;
+        };
+        // ---- the ring
         auto issue = [&](const uint8_t *tile, int stage) {
             if (tile != nullptr) {
                 const uint32_t to = ring_at + stage * Smem::BLOCK + 16 * lane;
@@ -130,38 +156,27 @@ __global__ void __launch_bounds__(kDigThreads, 2) kv_digits_kernel(const __grid_
         auto scales_of = [&](const uint8_t *tile) {
             return tile != nullptr ? __ldg(reinterpret_cast<const float2 *>(tile)) : make_float2(0.0f, 0.0f);
         };
-        int p = b0 + 2 * w;
-        const uint8_t *t0 = tile_at(p), *t1 = tile_at(p + 1);
+        const uint8_t *t0 = tile_at(p, 0), *t1 = tile_at(p + 1, 1);
+        const uint8_t *u0 = tile_at(p + 2 * kDigWarps, 2), *u1 = tile_at(p + 2 * kDigWarps + 1, 3);
         issue(t0, 0);
         issue(t1, 1);
-        const uint8_t *u0 = tile_at(p + 2 * kDigWarps), *u1 = tile_at(p + 2 * kDigWarps + 1);
         issue(u0, 2);
         issue(u1, 3);
         float2 sc0 = scales_of(t0), sc1 = scales_of(t1);
 
-        // ---- q of the columns, in digits
+        // ---- q in digits
         __syncthreads();  // the last task's join has read shared memory
-        for (int j = w; j < NC; j += kDigWarps) {
-            const int col = col0 + j;
-            constexpr int N = D / 32;
-            float x[N];
+        if (w < NC) {
             uint32_t mx = 0;
 #pragma unroll
-            for (int t = 0; t < N; ++t) x[t] = 0.0f;
-            if (col < cols) {
-                const int i = col / A.group;
-                load_row<N>(A.q, (size_t)(sq.a + i) * A.qs + ((size_t)h * A.group + (col - i * A.group)) * D + lane * N, A.type, x);
-            }
-#pragma unroll
-            for (int t = 0; t < N; ++t) mx = max(mx, __float_as_uint(x[t]) & 0x7fffffffu);
+            for (int t = 0; t < N; ++t) mx = max(mx, __float_as_uint(qx[t]) & 0x7fffffffu);
             mx = __reduce_max_sync(0xffffffffu, mx);
             // the largest |q| to [2^29, 2^30); a column that is not finite gets a scale that is NaN
             const int e = mx == 0 || mx >= 0x7f800000u ? 0 : min(120, 156 - (int)(mx >> 23));
             const float f = __int_as_float((127 + e) << 23);
 #pragma unroll
-            for (int t = 0; t < N; ++t) sm.q[j][lane * N + t] = digits_of(__float2int_rn(x[t] * f));
-            if (lane == 0)
-                sm.qscale[j] = mx >= 0x7f800000u ? __int_as_float(0x7fffffff) : (A.scale / f);
+            for (int t = 0; t < N; ++t) sm.q[w][lane * N + t] = digits_of(__float2int_rn(qx[t] * f));
+            if (lane == 0) sm.qscale[w] = mx >= 0x7f800000u ? __int_as_float(0x7fffffff) : A.scale * __int_as_float((127 - e) << 23);
         }
         for (int i = lane; i < NC * (D + 4); i += 32) sm.o[w][0][i] = 0.0f;
         __syncthreads();
@@ -193,10 +208,14 @@ __global__ void __launch_bounds__(kDigThreads, 2) kv_digits_kernel(const __grid_
         float m = -INFINITY, l = 0.0f, vref = 0x1p-100f;
         int held = 0;  // pairs in acc
         int half = 0;  // pair of the ring in work
-        for (; p < b1; p += 2 * kDigWarps, half ^= 1) {
-            // the tiles of the pair after the next one: their pages are asked for now
+        int k = 2;     // pair of `pages` after the next one
+        for (; p < b1; p += 2 * kDigWarps, half ^= 1, ++k) {
             const int pn = p + 4 * kDigWarps;
-            const uint8_t *const n0 = tile_at(pn), *const n1 = tile_at(pn + 1);
+            if (k == 16) {
+                pages = pages_from(pn);
+                k = 0;
+            }
+            const uint8_t *const n0 = tile_at(pn, 2 * k), *const n1 = tile_at(pn + 1, 2 * k + 1);
             const float2 sn0 = scales_of(u0), sn1 = scales_of(u1);
             asm volatile("cp.async.wait_group 2;" ::: "memory");
             const uint8_t *const st = ring + 2 * half * Smem::BLOCK;

@@ -76,6 +76,12 @@ __device__ __forceinline__ long long head_work(const AttnArgs &A, const Seq &q, 
     return mine;
 }
 
+// a / b; 64-bit divisions take a few hundred cycles
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    if (((a | b) >> 31) == 0) return (long long)((uint32_t)a / (uint32_t)b);
+    return a / b;
+}
+
 template <int WARPS>
 struct ShareSmem {
     long long sum[WARPS];
@@ -109,7 +115,7 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
         for (int i = 0; i < WARPS; ++i) total += sm.sum[i];
         __syncthreads();
     }
-    const long long share = max((long long)A.min_share, (total + gridDim.x - 1) / gridDim.x);
+    const long long share = max((long long)A.min_share, quotient(total + gridDim.x - 1, gridDim.x));
     const long long begin = share * blockIdx.x;
     if (begin >= total) return 0;
     if (threadIdx.x == 0) sm.share = share;
@@ -134,7 +140,7 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
             sm.seq = base + threadIdx.x;
             sm.rest = at;
             sm.q = q;
-            sm.head = mine / A.c.hk;
+            sm.head = quotient(mine, A.c.hk);
         }
         before += all;
         __syncthreads();
@@ -160,7 +166,7 @@ struct Walk {
     __device__ __forceinline__ Walk(const AttnArgs &a, int nc_, int shift_, long long left_, const Smem &sm)
         : A(a), nc(nc_), shift(shift_), left(left_), rest(sm.rest), share(sm.share), s(sm.seq), q(sm.q) {
         cols = q.n * A.group;
-        h = (int)(rest / sm.head);
+        h = (int)quotient(rest, sm.head);
         rest -= h * sm.head;
         col0 = -nc;
     }
@@ -179,7 +185,7 @@ struct Walk {
                         hw = head_work(A, q, nc, shift);
                     } while (hw == 0);
                     cols = q.n * A.group;
-                    h = (int)(rest / hw);
+                    h = (int)quotient(rest, hw);
                     rest -= h * hw;
                 }
             }
@@ -222,7 +228,7 @@ struct Walk {
     // the share ends inside a task that began in it: what the join needs
     __device__ __forceinline__ void note() const {
         A.rec[2 * blockIdx.x] = make_int4(1, q.a, cols, col0);
-        A.rec[2 * blockIdx.x + 1] = make_int4(h, (int)blockIdx.x + (int)((all - cnt + share - 1) / share), 0, 0);
+        A.rec[2 * blockIdx.x + 1] = make_int4(h, (int)blockIdx.x + (int)quotient(all - cnt + share - 1, share), 0, 0);
     }
     __device__ __forceinline__ bool open() const { return begins && !ends; }
 };
@@ -264,18 +270,21 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Joins the pieces of the task that began in CTA blockIdx.x's share and went on
-// in the next ones: one warp per column, blockIdx.y the eighth columns.
+// Joins the pieces of the task that began in CTA blockIdx.x's share and went on in the
+// next ones.  WIDE (many columns): one warp per column, blockIdx.y the eighth columns.
+// Else one CTA per column, blockIdx.y, whose warps take every eighth piece each: a long
+// sequence's few columns lie in tens of pieces, and their way is all that takes time.
 constexpr int kJoinWarps = 8;
-template <int D>
+template <int D, bool WIDE>
 __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_constant__ AttnArgs A, int nc) {
     constexpr int EPL = D / 32;
+    __shared__ float sum[kJoinWarps][D + 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 r0 = A.rec[2 * blockIdx.x];
+    const int4 r0 = A.rec[2 * blockIdx.x], r1 = A.rec[2 * blockIdx.x + 1];
     if (r0.x == 0) return;
-    const int4 r1 = A.rec[2 * blockIdx.x + 1];
-    const int j = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int j = WIDE ? blockIdx.y * kJoinWarps + w : blockIdx.y;
     const int col = r0.w + j;
     if (j >= nc || col >= r0.z) return;
     // piece 0: this CTA's second slot; then the first slots of the CTAs up to the task's last
@@ -283,6 +292,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_c
         return A.part + (size_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * part_floats(D, nc);
     };
     const int n = min(r1.y, (int)gridDim.x - 1) - (int)blockIdx.x + 1;
+    const int first = WIDE ? 0 : w, step = WIDE ? 1 : kJoinWarps;  // this warp's pieces
     // lane i holds the maximum and sum of piece i (of 32 at a time)
     float m = -INFINITY, l = 0.0f;
     if (lane < n) {
@@ -308,15 +318,17 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_c
         const float f = m == -INFINITY ? 1.0f : ex2(m - M);
         L = fmaf(f, l, L);
         const int cnt = min(32, n - base);
-        for (int i = 0; i < cnt; i += 8) {  // 8 pieces on their way
-            float y[8][EPL];
+        constexpr int AHEAD = WIDE ? 8 : 4;
+        for (int i = first; i < cnt; i += AHEAD * step) {  // pieces on their way
+            float y[AHEAD][EPL];
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (i + u < cnt) load_row<EPL>(piece(base + i + u), (size_t)j * D + lane * EPL, Q4RDNA_F32, y[u]);
+            for (int u = 0; u < AHEAD; ++u)
+                if (i + u * step < cnt)
+                    load_row<EPL>(piece(base + i + u * step), (size_t)j * D + lane * EPL, Q4RDNA_F32, y[u]);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float fu = __shfl_sync(0xffffffffu, f, (i + u) & 31);
-                if (i + u < cnt)
+            for (int u = 0; u < AHEAD; ++u) {
+                const float fu = __shfl_sync(0xffffffffu, f, (i + u * step) & 31);
+                if (i + u * step < cnt)
 #pragma unroll
                     for (int t = 0; t < EPL; ++t) x[t] = fmaf(fu, y[u][t], x[t]);
             }
@@ -324,6 +336,18 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_c
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if constexpr (!WIDE) {
+#pragma unroll
+        for (int t = 0; t < EPL; ++t) sum[w][lane * EPL + t] = x[t];
+        __syncthreads();
+        if (w > 0) return;
+#pragma unroll
+        for (int t = 0; t < EPL; ++t) x[t] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kJoinWarps; ++i)
+#pragma unroll
+            for (int t = 0; t < EPL; ++t) x[t] += sum[i][lane * EPL + t];
+    }
     const float r = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
     for (int t = 0; t < EPL; ++t) x[t] *= r;
