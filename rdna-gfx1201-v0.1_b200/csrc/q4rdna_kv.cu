@@ -12,7 +12,6 @@
 #include "q4rdna_kv.h"
 #include "q4rdna_kv_append.cuh"
 #include "q4rdna_kv_attention.cuh"
-#include "q4rdna_kv_digits.cuh"
 #include "q4rdna_kv_tile.cuh"
 
 namespace q4 {
@@ -188,10 +187,6 @@ Variant variant(int format, int nt, int terms) {
     return format == Q4RDNA_KV_INT8 ? variant<D, Q4RDNA_KV_INT8>(nt, terms) : variant<D, Q4RDNA_KV_E4M3>(nt, terms);
 }
 template <int D>
-Variant digits_variant() {
-    return {kv_digits_kernel<D>, sizeof(DigSmem<D>), kDigThreads, kDigCols, 4};
-}
-template <int D>
 Variant tile32_variant(int format) {
     return {format == Q4RDNA_KV_INT8 ? kv_tile32_kernel<D, Q4RDNA_KV_INT8> : kv_tile32_kernel<D, Q4RDNA_KV_E4M3>,
             sizeof(TileSmem<D>), kTileThreads, kTile32Cols, kTileShift};
@@ -258,13 +253,11 @@ q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &
         // one column tile where a token's heads fit it and each sequence has one token, else two
         const int nt = A.b.q_start == nullptr && A.group <= 8 ? 1 : 2, terms = A.type == Q4RDNA_F32 ? 2 : 1;
         AttnLaunch &l = L[n++];
-        const int dg = getenv("DG") ? atoi(getenv("DG")) : 4;
-        if (A.c.format == Q4RDNA_KV_INT8 && D <= 128 && most <= dg) l.v = D == 64 ? digits_variant<64>() : digits_variant<128>();
-        else l.v = D == 64 ? variant<64>(A.c.format, nt, terms)
+        l.v = D == 64 ? variant<64>(A.c.format, nt, terms)
                       : D == 128 ? variant<128>(A.c.format, nt, terms) : variant<256>(A.c.format, nt, terms);
         l.few = 0;
         l.many = tiles ? from : INT_MAX;
-        l.min_share = l.v.nc == kDigCols ? 2 * kDigWarps : kAttnWarps;  // one block per warp (or a pair)
+        l.min_share = kAttnWarps;  // one block per warp
     }
     if (tiles) {
         AttnLaunch &l = L[n++];
