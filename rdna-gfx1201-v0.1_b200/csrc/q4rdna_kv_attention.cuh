@@ -112,9 +112,71 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
     bool open = false;  // the share ends inside a task that began in it
     const int t0 = 4 * (g >> 1) + (g & 1);  // K rows g and g + 8 of the fragments: tokens t0 and t0 + 2
     Walk W(A, NC, 4, left, sm.share);
-    while (W.next()) {
-        const Seq &sq = W.q;
-        const int s = W.s, cols = W.cols, h = W.h, col0 = W.col0, b0 = W.begin, b1 = W.end;
+
+    uint4 kr[2][KW];
+    uint32_t vr[4][VB / 4];
+    float2 sc = make_float2(0.0f, 0.0f);
+    auto load_k = [&](const uint8_t *tile) {
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+            kr[0][i] = ld_stream(tile + kHeader + t0 * D + 16 * c + 64 * i);
+            kr[1][i] = ld_stream(tile + kHeader + (t0 + 2) * D + 16 * c + 64 * i);
+        }
+    };
+    auto load_v = [&](const uint8_t *tile) {
+        const uint8_t *p = tile + kHeader + (kBlock + 4 * c) * D + VB * g;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if constexpr (VB == 8) {
+                const uint2 x = ld_stream2(p + t * D);
+                vr[t][0] = x.x; vr[t][1] = x.y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VB / 16; ++i) {
+                    const uint4 x = ld_stream(p + t * D + 16 * i);
+                    vr[t][4 * i] = x.x; vr[t][4 * i + 1] = x.y; vr[t][4 * i + 2] = x.z; vr[t][4 * i + 3] = x.w;
+                }
+            }
+        }
+    };
+    // This warp's blocks are b, b + kAttnWarps, ...; lane i holds the page of the i-th of 32,
+    // so that the loop waits for no page table
+    int b = 0, at = 0, pages = 0;
+    const uint8_t *tile = nullptr;
+    auto fetch_pages = [&]() {
+        const int blk = b + kAttnWarps * lane;
+        pages = blk < W.end ? B.table[(size_t)W.s * B.stride + (blk >> A.c.nbl)] : 0;
+        at = 0;
+    };
+    // the next block of this warp, from b on, whose page lies in the cache
+    auto next_tile = [&]() -> const uint8_t * {
+        for (; b < W.end; b += kAttnWarps, ++at) {
+            if (at == 32) fetch_pages();
+            const int page = __shfl_sync(0xffffffffu, pages, at);
+            if ((unsigned)page < (unsigned)A.c.pages) {
+                const size_t t = (((size_t)page * A.c.hk + W.h) << A.c.nbl) + (b & ((1 << A.c.nbl) - 1));
+                return A.c.tiles + t * A.c.tile_bytes;
+            }
+            if (lane == 0) atomicOr(&g_kv_fault, kFaultBatch);
+        }
+        return nullptr;
+    };
+    // a task's first block on its way
+    auto enter = [&]() {
+        b = W.begin + w;
+        fetch_pages();
+        tile = next_tile();
+        if (tile != nullptr) {
+            load_k(tile);
+            load_v(tile);
+            sc = __ldg(reinterpret_cast<const float2 *>(tile));
+        }
+    };
+    bool more = W.next();
+    if (more) enter();
+    while (more) {
+        const Seq sq = W.q;
+        const int cols = W.cols, h = W.h, col0 = W.col0;
         const int first = sq.L - sq.n;  // token of the sequence's first row
 
         // ---- q of the columns, scaled to f16
@@ -178,51 +240,11 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
         const int full_hi = (first + col0 / A.group + 1) >> 4;  // first block that is not whole below
         const int full_lo = A.window > 0 ? (max(0, last - A.window + 1) + 15) >> 4 : 0;
 
-        uint4 kr[2][KW];
-        uint32_t vr[4][VB / 4];
-        float2 sc = make_float2(0.0f, 0.0f);
-        auto load_k = [&](const uint8_t *tile) {
-#pragma unroll
-            for (int i = 0; i < KW; ++i) {
-                kr[0][i] = ld_stream(tile + kHeader + t0 * D + 16 * c + 64 * i);
-                kr[1][i] = ld_stream(tile + kHeader + (t0 + 2) * D + 16 * c + 64 * i);
-            }
-        };
-        auto load_v = [&](const uint8_t *tile) {
-            const uint8_t *p = tile + kHeader + (kBlock + 4 * c) * D + VB * g;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                if constexpr (VB == 8) {
-                    const uint2 x = ld_stream2(p + t * D);
-                    vr[t][0] = x.x; vr[t][1] = x.y;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < VB / 16; ++i) {
-                        const uint4 x = ld_stream(p + t * D + 16 * i);
-                        vr[t][4 * i] = x.x; vr[t][4 * i + 1] = x.y; vr[t][4 * i + 2] = x.z; vr[t][4 * i + 3] = x.w;
-                    }
-                }
-            }
-        };
-        // the next block of this warp whose page lies in the cache
-        auto next_tile = [&](int &b) -> const uint8_t * {
-            for (; b < b1; b += kAttnWarps) {
-                const uint8_t *t = tile_of(A.c, B, s, h, b);
-                if (t != nullptr) return t;
-            }
-            return nullptr;
-        };
-        int b = b0 + w;
-        const uint8_t *tile = next_tile(b);
-        if (tile != nullptr) {
-            load_k(tile);
-            load_v(tile);
-            sc = __ldg(reinterpret_cast<const float2 *>(tile));
-        }
         while (tile != nullptr) {
             const int cur = b;
             b += kAttnWarps;
-            const uint8_t *next = next_tile(b);
+            ++at;
+            const uint8_t *next = next_tile();
 
             // scores
             float sa[NT][TERMS][4];
@@ -384,9 +406,15 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
                     *reinterpret_cast<float2 *>(&sm.o[w][j][VB * g + 2 * i]) =
                         make_float2(o[n][i][z], o[n][i][z + 2]);
             }
-        __syncthreads();
         const bool whole_task = W.whole();
         float *part = W.part(D);
+        if (W.open()) {
+            open = true;
+            if (threadIdx.x == 0) W.note();
+        }
+        more = W.next();
+        if (more) enter();  // while this task's results meet
+        __syncthreads();
         for (int e = threadIdx.x; e < NC * (D / 4); e += kAttnThreads) {
             const int j = e / (D / 4), d = 4 * (e % (D / 4));
             const int col = col0 + j;
@@ -420,10 +448,6 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
                     part[NC * D + NC + j] = L;
                 }
             }
-        }
-        if (W.open()) {
-            open = true;
-            if (threadIdx.x == 0) W.note();
         }
     }
     if (threadIdx.x == 0 && !open) A.rec[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
