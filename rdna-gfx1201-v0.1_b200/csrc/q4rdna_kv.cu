@@ -239,8 +239,8 @@ q4rdna_status size_launch(const AttnArgs &A, int D, AttnLaunch &L) {
 }
 
 // Columns from which on the tile kernels take a sequence
-const int kTileFrom = getenv("TF") ? atoi(getenv("TF")) : 48;
-const int kTile32From = getenv("TF32") ? atoi(getenv("TF32")) : 48;
+const int kTileFrom = getenv("TF") ? atoi(getenv("TF")) : 96;
+const int kTile32From = getenv("TF32") ? atoi(getenv("TF32")) : 96;
 
 // The launches of a call: sequences of few columns, sequences of many, or both
 q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &n) {
@@ -249,7 +249,9 @@ q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &
     const bool f32 = A.type == Q4RDNA_F32;
     const int from = f32 ? kTile32From : kTileFrom;
     const bool tiles = D <= 128 && most >= from;
-    if (!tiles || (A.b.S > 1 && A.b.q_start != nullptr)) {
+    // (one sequence, or a few of many columns on average: no launch for the others, which the tile kernels take too)
+    const bool alone = A.b.S == 1 || A.b.q_start == nullptr || (A.b.S <= 4 && most >= 4LL * from * A.b.S);
+    if (!tiles || !alone) {
         // one column tile where a token's heads fit it and each sequence has one token, else two
         const int nt = A.b.q_start == nullptr && A.group <= 8 ? 1 : 2, terms = A.type == Q4RDNA_F32 ? 2 : 1;
         AttnLaunch &l = L[n++];

@@ -91,7 +91,7 @@ struct AttnSmem {
 };
 
 template <int D, int FMT, int NT, int TERMS>
-__global__ void __launch_bounds__(kAttnThreads, NT == 1 && D <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(kAttnThreads, D == 64 || (NT == 1 && D == 128) ? 2 : 1)
 kv_attention_kernel(const __grid_constant__ AttnArgs A) {
     using Smem = AttnSmem<D, NT>;
     constexpr int NC = Smem::NC, KW = D / 64;  // KW: 16-byte loads of a K row per lane

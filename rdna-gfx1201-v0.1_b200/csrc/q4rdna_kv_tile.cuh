@@ -149,7 +149,21 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&v)[16]) {
           "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for the loads; the registers are named, so that nothing that reads them comes first
+__device__ __forceinline__ void tmem_arrived(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                   "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
+                   "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]),
+                   "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]),
+                   "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                   "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
+                   "+r"(v[14]), "+r"(v[15]));
+}
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
     asm volatile(
@@ -204,7 +218,7 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 tmem_load32(s_at + 32 * c, v);
-                tmem_wait_load();
+                tmem_arrived(v);
                 const int tok = tok0 + 32 * c;
                 if (tok < all_lo || tok + 31 > all_hi) {
 #pragma unroll
@@ -229,7 +243,7 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     tmem_load32(o_at + c, v);
-                    tmem_wait_load();
+                    tmem_arrived(v);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
                     tmem_store32(o_at + c, v);
@@ -246,7 +260,7 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
 #pragma unroll
         for (int b = 0; b < 9; ++b) {
             if (b < 8) {
-                tmem_wait_load();
+                tmem_arrived(v[b & 1]);
                 if (b < 7) tmem_load16(s_at + 16 * (b + 1), v[(b + 1) & 1]);
                 const float4 g = scale[b];
                 const float a = g.x * r.scale, d = g.y - ref;
@@ -709,7 +723,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                         uint32_t v[32];
                         if (steps > 0) {
                             tmem_load32(o_at + c, v);
-                            tmem_wait_load();
+                            tmem_arrived(v);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = 0;
@@ -798,7 +812,7 @@ __device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
             tmem_load32(s_at + 32 * c, v);
-            tmem_wait_load();
+            tmem_arrived(v);
             hide(tok0 + 32 * c);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -821,7 +835,7 @@ __device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm
         for (int c = 0; c < 4; ++c) {
             uint32_t p[32];
             tmem_load32(s_at + 32 * c, v);
-            tmem_wait_load();
+            tmem_arrived(v);
             const int tok = tok0 + 32 * c;
             const bool part = tok < all_lo || tok + 31 > all_hi;
 #pragma unroll
@@ -902,7 +916,8 @@ __device__ __noinline__ bool add32_rows(const AttnArgs &A, const Walk &W, TileSm
             if (steps > 0) {
                 tmem_load32(step_at + c, v);
                 if (j > 0) tmem_load32(o_at + c, u);
-                tmem_wait_load();
+                tmem_arrived(v);
+                tmem_arrived(u);
             }
             if (j > 0) {
 #pragma unroll
