@@ -349,8 +349,8 @@ q4rdna_status q4rdna_pack_bf16(const uint16_t *bf16, uint8_t *tiles, int N, int 
  * `pages` pages back to back, 16-byte aligned.  Token p of sequence s lives in
  * page page_table[s * table_stride + p / page_tokens], tile p % page_tokens / 16,
  * row p % 16.  head_dim is 64, 128 or 256; page_tokens a power of two in
- * [16, 256].  A tile whose numbers are all below 2^-100 of the largest code is
- * stored as zeros with scale 0. */
+ * [16, 256].  A tile whose scale would be below 2^-100 is stored as zeros with
+ * scale 0. */
 #define Q4RDNA_KV_BLOCK 16
 typedef enum q4rdna_kv_format { Q4RDNA_KV_INT8 = 0, Q4RDNA_KV_E4M3 = 1 } q4rdna_kv_format;
 /* Element type of q, k, v and the outputs of the cache operators. */
@@ -374,7 +374,8 @@ typedef struct q4rdna_kv_cache {
  * ones.  A negative token (a padded row of a batch: lengths[s] < n) is not
  * stored and sees nothing.  The arrays are device memory and are read when the
  * kernels run, so a captured call takes the values of the replay.  max_length
- * (0: table_stride * page_tokens) bounds every length on the host's side. */
+ * (0: table_stride * page_tokens, at most 2^30) bounds every length on the
+ * host's side. */
 typedef struct q4rdna_kv_batch {
     const int32_t *page_table; /* [sequences][table_stride] */
     const int32_t *lengths;    /* [sequences] */
@@ -434,8 +435,10 @@ q4rdna_status q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_bat
 
 /* out = softmax(scale * q k^T) v over the cached tokens that the row's token
  * sees: those up to itself, at most `window` of them.  A row that sees nothing
- * becomes 0; rows outside every sequence keep their values.  Accumulation in
- * f32.  The workspace (q4rdna_kv_attention_workspace_bytes, 16-byte aligned)
+ * becomes 0; rows outside every sequence keep their values.  f32 rows are
+ * computed in at least 22 bits (two f16 terms of q and of the weights, sums in
+ * f32), 16-bit rows with weights in f16; results do not depend on the timing.
+ * The workspace (q4rdna_kv_attention_workspace_bytes, 16-byte aligned)
  * needs no initialisation and carries nothing from call to call; calls that
  * may overlap on the GPU need one each. */
 q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,

@@ -4,7 +4,6 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
-#include <cstdlib>
 #include <map>
 #include <mutex>
 #include <set>
@@ -44,7 +43,7 @@ q4rdna_status check_batch(const q4rdna_kv_cache *c, const q4rdna_kv_batch *b, in
     if (b == nullptr || b->page_table == nullptr || b->lengths == nullptr) return Q4RDNA_ERR_INVALID_ARGUMENT;
     if (b->sequences < 0 || b->table_stride <= 0 || b->max_length < 0 || tokens < 0) return Q4RDNA_ERR_INVALID_ARGUMENT;
     if (b->q_start == nullptr && tokens != b->sequences) return Q4RDNA_ERR_SHAPE;
-    const long long room = std::min<long long>((long long)b->table_stride * c->page_tokens, INT_MAX - 256);
+    const long long room = std::min<long long>((long long)b->table_stride * c->page_tokens, 1 << 30);
     if (b->max_length > room) return Q4RDNA_ERR_SHAPE;
     // the append's units and the attention's 32-bit row arithmetic
     if (b->sequences > (1 << 28) || tokens > (1 << 28)) return Q4RDNA_ERR_TOO_LARGE;
@@ -120,7 +119,8 @@ q4rdna_status check_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_batc
     A.group = args->heads / cache->kv_heads;
     const float scale = args->scale > 0.0f ? args->scale : 1.0f / std::sqrt((float)D);
     A.scale = scale * 1.44269504088896340736f;
-    A.window = args->window;
+    A.window = args->window < A.b.max_len ? args->window : 0;
+    if ((long long)args->tokens * A.group > (1 << 30)) return Q4RDNA_ERR_TOO_LARGE;  // columns of a kv head
     return Q4RDNA_OK;
 }
 
@@ -238,19 +238,22 @@ q4rdna_status size_launch(const AttnArgs &A, int D, AttnLaunch &L) {
     return Q4RDNA_OK;
 }
 
-// Columns from which on the tile kernels take a sequence
-const int kTileFrom = getenv("TF") ? atoi(getenv("TF")) : 96;
-const int kTile32From = getenv("TF32") ? atoi(getenv("TF32")) : 96;
+// Columns (new tokens x query heads of a kv head) from which on the tile kernels take a
+// sequence.  Measured with 32 query and 8 kv heads of 128, int8, one or four sequences, us
+// for the kernel for few columns and for the tile kernel:
+//   columns             16       32       48       64      128      256     2048
+//   f32              28, 56   40, 58   51, 60   63, 62   81, 59   84, 53  350, 136
+//   bf16             26, 56   35, 58   44, 59   53, 60   66, 51   70, 47  272, 89
+constexpr int kTileFrom = 96;
 
 // The launches of a call: sequences of few columns, sequences of many, or both
 q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &n) {
     n = 0;
     const long long most = A.b.q_start == nullptr ? A.group : (long long)A.b.T * A.group;  // columns of a sequence
     const bool f32 = A.type == Q4RDNA_F32;
-    const int from = f32 ? kTile32From : kTileFrom;
-    const bool tiles = D <= 128 && most >= from;
+    const bool tiles = D <= 128 && most >= kTileFrom;
     // (one sequence, or a few of many columns on average: no launch for the others, which the tile kernels take too)
-    const bool alone = A.b.S == 1 || A.b.q_start == nullptr || (A.b.S <= 4 && most >= 4LL * from * A.b.S);
+    const bool alone = A.b.S == 1 || A.b.q_start == nullptr || (A.b.S <= 4 && most >= 4LL * kTileFrom * A.b.S);
     if (!tiles || !alone) {
         // one column tile where a token's heads fit it and each sequence has one token, else two
         const int nt = A.b.q_start == nullptr && A.group <= 8 ? 1 : 2, terms = A.type == Q4RDNA_F32 ? 2 : 1;
@@ -258,14 +261,14 @@ q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &
         l.v = D == 64 ? variant<64>(A.c.format, nt, terms)
                       : D == 128 ? variant<128>(A.c.format, nt, terms) : variant<256>(A.c.format, nt, terms);
         l.few = 0;
-        l.many = tiles ? from : INT_MAX;
+        l.many = tiles ? kTileFrom : INT_MAX;
         l.min_share = kAttnWarps;  // one block per warp
     }
     if (tiles) {
         AttnLaunch &l = L[n++];
         if (f32) l.v = D == 64 ? tile32_variant<64>(A.c.format) : tile32_variant<128>(A.c.format);
         else l.v = D == 64 ? tile_variant<64>(A.c.format) : tile_variant<128>(A.c.format);
-        l.few = n == 2 ? from : 0;
+        l.few = n == 2 ? kTileFrom : 0;
         l.many = INT_MAX;
         l.min_share = 2;
     }

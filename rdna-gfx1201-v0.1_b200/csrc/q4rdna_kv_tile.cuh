@@ -622,8 +622,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Bars bar{smem_u32(sm.bar)};
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = tile_enter<D>(sm, bar);
+    // only now: a dependent kernel that takes tensor memory must not come before this CTA
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const long long left = find_share<kTileWarps>(A, kTileCols, kTileShift, sm.share);
@@ -1016,8 +1017,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile32_kernel(const __grid
     Smem &sm = *reinterpret_cast<Smem *>(tile_smem);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Bars bar{smem_u32(sm.bar)};
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = tile_enter<D>(sm, bar);
+    // only now: a dependent kernel that takes tensor memory must not come before this CTA
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const long long left = find_share<kTileWarps>(A, kTile32Cols, kTileShift, sm.share);

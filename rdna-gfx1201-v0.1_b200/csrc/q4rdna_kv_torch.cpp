@@ -128,7 +128,7 @@ q4rdna_kv_batch batch_for(const BatchRec &b, const CacheRec &c) {
                       std::to_string(room) + " tokens");
     if (b.device != c.device) throw Refused("kv cache operators: the batch is on another device than the cache");
     q4rdna_kv_batch d = b.desc;
-    d.max_length = b.limit > 0 ? b.limit : (int)std::min<int64_t>(room, INT_MAX - 256);
+    d.max_length = b.limit > 0 ? b.limit : (int)std::min<int64_t>(room, 1 << 30);
     return d;
 }
 

@@ -175,3 +175,12 @@ def test_python_refusals_by_shape_come_before_the_device():
         q4rdna.kv_append(cache, batch, torch.zeros((3, 3, 64)), torch.zeros((3, 2, 64)))
     with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
         q4rdna.kv_attention(cache, batch, torch.zeros((3, 2, 64), dtype=torch.int8))
+
+
+def test_columns_past_32_bits_are_refused():
+    """Rows times query heads of a kv head is an int in the kernels."""
+    n, h = 1 << 26, 64
+    c, b = refs(desc(kv_heads=1), batch(sequences=n))
+    args = dict(tokens=n, heads=h, q_stride=h * 128, out_stride=h * 128)
+    assert q4rdna.lib.q4rdna_kv_attention(c, b, *refs(attention_args(**args)), A, 1 << 40, None) == TOO_LARGE
+    assert q4rdna.lib.q4rdna_kv_attention_workspace_bytes(c, b, *refs(attention_args(**args))) == 0
