@@ -406,12 +406,10 @@ q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_
         at += l.workspace;
         if ((st = launch(l.v.kernel, dim3(l.grid), l.v.threads, l.v.smem, cs, A)) != Q4RDNA_OK) return st;
         const bool wide = l.v.nc > 16;
-        const auto join = D == 64    ? (wide ? kv_join_kernel<64, true> : kv_join_kernel<64, false>)
-                          : D == 128 ? (wide ? kv_join_kernel<128, true> : kv_join_kernel<128, false>)
-                                     : (wide ? kv_join_kernel<256, true> : kv_join_kernel<256, false>);
-        if ((st = launch(join, dim3(l.grid, (unsigned)(wide ? l.v.nc / kJoinWarps : l.v.nc)), 32 * kJoinWarps, 0, cs, A,
-                         l.v.nc)) != Q4RDNA_OK)
-            return st;
+        const auto join = wide ? (D == 64 ? kv_join_wide_kernel<64> : kv_join_wide_kernel<128>)
+                               : (D == 64 ? kv_join_kernel<64> : D == 128 ? kv_join_kernel<128> : kv_join_kernel<256>);
+        const unsigned y = (unsigned)(wide ? l.v.nc / (kJoinWarps * kJoinCols) : l.v.nc);
+        if ((st = launch(join, dim3(l.grid, y), 32 * kJoinWarps, 0, cs, A, l.v.nc)) != Q4RDNA_OK) return st;
     }
     return Q4RDNA_OK;
 }

@@ -112,7 +112,10 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
         for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
         if (lane == 0) sm.sum[w] = x;
         __syncthreads();
-        for (int i = 0; i < WARPS; ++i) total += sm.sum[i];
+        x = lane < WARPS ? sm.sum[lane] : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        total += x;
         __syncthreads();
     }
     const long long share = max((long long)A.min_share, quotient(total + gridDim.x - 1, gridDim.x));
@@ -130,11 +133,13 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
         }
         if (lane == 31) sm.sum[w] = x;
         __syncthreads();
-        long long all = 0;
-        for (int i = 0; i < WARPS; ++i) {
-            if (i < w) x += sm.sum[i];
-            all += sm.sum[i];
+        long long ahead = lane < w ? sm.sum[lane] : 0, all = lane < WARPS ? sm.sum[lane] : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+            all += __shfl_xor_sync(0xffffffffu, all, o);
         }
+        x += ahead;
         const long long at = begin - before - (x - mine);
         if (at >= 0 && at < mine) {
             sm.seq = base + threadIdx.x;
@@ -271,64 +276,77 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
 }
 
 // Joins the pieces of the task that began in CTA blockIdx.x's share and went on in the
-// next ones.  WIDE (many columns): one warp per column, blockIdx.y the eighth columns.
-// Else one CTA per column, blockIdx.y, whose warps take every eighth piece each: a long
-// sequence's few columns lie in tens of pieces, and their way is all that takes time.
+// next ones: bound by the latency of a few dependent loads, so as many as can be are on
+// their way together.
+
 constexpr int kJoinWarps = 8;
-template <int D, bool WIDE>
+
+// Where the pieces of a record lie
+struct Pieces {
+    const float *part;
+    int nc, n;  // columns of a task; pieces
+    size_t floats;
+    // piece 0: this CTA's second slot; then the first slots of the CTAs up to the task's last
+    __device__ __forceinline__ const float *operator()(int i) const {
+        return part + (size_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * floats;
+    }
+};
+template <int D>
+__device__ __forceinline__ Pieces pieces_of(const AttnArgs &A, int nc, int last) {
+    return {A.part, nc, min(last, (int)gridDim.x - 1) - (int)blockIdx.x + 1, (size_t)part_floats(D, nc)};
+}
+template <int EPL>
+__device__ __forceinline__ void store_column(const AttnArgs &A, const int4 &r0, int h, int col, float L, float (&x)[EPL]) {
+    const float r = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int t = 0; t < EPL; ++t) x[t] *= r;
+    const int i = col / A.group, lane = threadIdx.x & 31;
+    store_row<EPL>(A.out,
+                   (size_t)(r0.y + i) * A.os + ((size_t)h * A.group + (col - i * A.group)) * (32 * EPL) + lane * EPL, A.type, x);
+}
+
+// Few columns: one CTA per column, blockIdx.y, whose warps take every eighth piece each
+// (a long sequence's few columns lie in tens of pieces)
+template <int D>
 __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_constant__ AttnArgs A, int nc) {
-    constexpr int EPL = D / 32;
+    constexpr int EPL = D / 32, AHEAD = 4;
     __shared__ float sum[kJoinWarps][D + 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 r0 = A.rec[2 * blockIdx.x], r1 = A.rec[2 * blockIdx.x + 1];
     if (r0.x == 0) return;
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int j = WIDE ? blockIdx.y * kJoinWarps + w : blockIdx.y;
-    const int col = r0.w + j;
-    if (j >= nc || col >= r0.z) return;
-    // piece 0: this CTA's second slot; then the first slots of the CTAs up to the task's last
-    auto piece = [&](int i) {
-        return A.part + (size_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * part_floats(D, nc);
-    };
-    const int n = min(r1.y, (int)gridDim.x - 1) - (int)blockIdx.x + 1;
-    const int first = WIDE ? 0 : w, step = WIDE ? 1 : kJoinWarps;  // this warp's pieces
+    const int j = blockIdx.y, col = r0.w + j;
+    if (col >= r0.z) return;
+    const Pieces piece = pieces_of<D>(A, nc, r1.y);
+    const int n = piece.n;
     // lane i holds the maximum and sum of piece i (of 32 at a time)
-    float m = -INFINITY, l = 0.0f;
-    if (lane < n) {
-        m = piece(lane)[nc * D + j];
-        l = piece(lane)[nc * D + nc + j];
-    }
-    float M = m;
-    for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, piece(i)[nc * D + j]);
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, piece(i)[nc * D + j]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float x[EPL], L = 0.0f;
 #pragma unroll
     for (int t = 0; t < EPL; ++t) x[t] = 0.0f;
     for (int base = 0; base < n; base += 32) {
-        if (base > 0) {
-            m = -INFINITY;
-            l = 0.0f;
-            if (base + lane < n) {
-                m = piece(base + lane)[nc * D + j];
-                l = piece(base + lane)[nc * D + nc + j];
-            }
+        float m = -INFINITY, l = 0.0f;
+        if (base + lane < n) {
+            m = piece(base + lane)[nc * D + j];
+            l = piece(base + lane)[nc * D + nc + j];
         }
         const float f = m == -INFINITY ? 1.0f : ex2(m - M);
         L = fmaf(f, l, L);
         const int cnt = min(32, n - base);
-        constexpr int AHEAD = WIDE ? 8 : 4;
-        for (int i = first; i < cnt; i += AHEAD * step) {  // pieces on their way
+        for (int i = w; i < cnt; i += AHEAD * kJoinWarps) {
             float y[AHEAD][EPL];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u)
-                if (i + u * step < cnt)
-                    load_row<EPL>(piece(base + i + u * step), (size_t)j * D + lane * EPL, Q4RDNA_F32, y[u]);
+                if (i + u * kJoinWarps < cnt)
+                    load_row<EPL>(piece(base + i + u * kJoinWarps), (size_t)j * D + lane * EPL, Q4RDNA_F32, y[u]);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const float fu = __shfl_sync(0xffffffffu, f, (i + u * step) & 31);
-                if (i + u * step < cnt)
+                const float fu = __shfl_sync(0xffffffffu, f, (i + u * kJoinWarps) & 31);
+                if (i + u * kJoinWarps < cnt)
 #pragma unroll
                     for (int t = 0; t < EPL; ++t) x[t] = fmaf(fu, y[u][t], x[t]);
             }
@@ -336,24 +354,81 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_c
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if constexpr (!WIDE) {
 #pragma unroll
-        for (int t = 0; t < EPL; ++t) sum[w][lane * EPL + t] = x[t];
-        __syncthreads();
-        if (w > 0) return;
+    for (int t = 0; t < EPL; ++t) sum[w][lane * EPL + t] = x[t];
+    __syncthreads();
+    if (w > 0) return;
 #pragma unroll
-        for (int t = 0; t < EPL; ++t) x[t] = 0.0f;
+    for (int t = 0; t < EPL; ++t) x[t] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kJoinWarps; ++i)
+    for (int i = 0; i < kJoinWarps; ++i)
 #pragma unroll
-            for (int t = 0; t < EPL; ++t) x[t] += sum[i][lane * EPL + t];
+        for (int t = 0; t < EPL; ++t) x[t] += sum[i][lane * EPL + t];
+    store_column<EPL>(A, r0, r1.x, col, L, x);
+}
+
+// Many columns: a warp takes four of them together, all pieces; blockIdx.y the 32 columns
+constexpr int kJoinCols = 4;
+template <int D>
+__global__ void __launch_bounds__(32 * kJoinWarps) kv_join_wide_kernel(const __grid_constant__ AttnArgs A, int nc) {
+    constexpr int EPL = D / 32, AHEAD = 4;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 r0 = A.rec[2 * blockIdx.x], r1 = A.rec[2 * blockIdx.x + 1];
+    if (r0.x == 0) return;
+    const int lane = threadIdx.x & 31;
+    const int j0 = (blockIdx.y * kJoinWarps + (threadIdx.x >> 5)) * kJoinCols;
+    if (r0.w + j0 >= r0.z) return;
+    const Pieces piece = pieces_of<D>(A, nc, r1.y);
+    const int n = piece.n, cols = min(kJoinCols, r0.z - r0.w - j0);
+    // lane 8 k + i holds the maximum and sum of piece i (of 8 at a time) of column k
+    const int k = lane >> 3, i = lane & 7;
+    const bool there = k < cols;
+    float M = -INFINITY;
+    for (int b = i; b < n && there; b += 8) M = fmaxf(M, piece(b)[nc * D + j0 + k]);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float x[kJoinCols][EPL], L = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kJoinCols; ++c)
+#pragma unroll
+        for (int t = 0; t < EPL; ++t) x[c][t] = 0.0f;
+    for (int base = 0; base < n; base += 8) {
+        float m = -INFINITY, l = 0.0f;
+        if (base + i < n && there) {
+            m = piece(base + i)[nc * D + j0 + k];
+            l = piece(base + i)[nc * D + nc + j0 + k];
+        }
+        const float f = m == -INFINITY ? 1.0f : ex2(m - M);
+        L = fmaf(f, l, L);
+#pragma unroll
+        for (int u0 = 0; u0 < 8; u0 += AHEAD) {
+            if (base + u0 >= n) break;
+            float y[AHEAD][kJoinCols][EPL];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int c = 0; c < kJoinCols; ++c)
+                    if (base + u0 + u < n && c < cols)
+                        load_row<EPL>(piece(base + u0 + u), (size_t)(j0 + c) * D + lane * EPL, Q4RDNA_F32, y[u][c]);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int c = 0; c < kJoinCols; ++c) {
+                    const float fu = __shfl_sync(0xffffffffu, f, 8 * c + u0 + u);
+                    if (base + u0 + u < n && c < cols)
+#pragma unroll
+                        for (int t = 0; t < EPL; ++t) x[c][t] = fmaf(fu, y[u][c][t], x[c][t]);
+                }
+        }
     }
-    const float r = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-    for (int t = 0; t < EPL; ++t) x[t] *= r;
-    const int i = col / A.group;
-    store_row<EPL>(A.out, (size_t)(r0.y + i) * A.os + ((size_t)r1.x * A.group + (col - i * A.group)) * D + lane * EPL, A.type,
-                   x);
+    for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+#pragma unroll
+    for (int c = 0; c < kJoinCols; ++c) {
+        const float Lc = __shfl_sync(0xffffffffu, L, 8 * c);
+        if (c < cols) store_column<EPL>(A, r0, r1.x, r0.w + j0 + c, Lc, x[c]);
+    }
 }
 
 }  // namespace q4kv
