@@ -976,6 +976,130 @@ def run_reference(args):
     }
 
 
+# ------------------------------------------------- decode step with attention
+
+HEAD_DIM = 128  # of the Qwen3 models
+
+
+def run_attention(args):
+    """One whole decoder step of --batch sequences that hold --attention tokens
+    each: per layer the q/k/v products (RMSNorm fused), the append to the 8-bit
+    cache with per-head norms and rotation, the attention, the output product +
+    residual, gate/up (SwiGLU, RMSNorm fused) and the down product + residual,
+    each reading what the one before wrote; one CUDA graph per step.  Timed as a
+    whole, and the layers' products and the appends + attentions alone."""
+    import torch
+
+    import q4rdna
+    from q4rdna import synth
+
+    dev, B, ctx = torch.device("cuda", 0), args.batch, args.attention
+    torch.cuda.set_device(dev)
+    peak, src = hbm_peak()
+    g = torch.Generator(device=dev)
+    g.manual_seed(args.seed)
+    names = synth.model_tensors(args.model)
+    if args.layers:
+        names = [t for t in names if int(t[0].split(".")[1]) < args.layers]
+    per = 1 + max(int(n.split(".")[1]) for n, _, _ in names)
+    shape = {n.split(".")[2]: (N, K) for n, N, K in names}
+    hid, D, P = shape["attn_q"][1], HEAD_DIM, 64
+    heads, kvh = shape["attn_q"][0] // D, shape["attn_k"][0] // D
+    new = lambda rows: torch.empty((B, rows), dtype=torch.float32, device=dev)
+    x0 = new(hid).normal_(generator=g)
+    h, mid, act = new(hid), new(hid), new(shape["ffn_gate"][0])
+    qkv = {n: new(shape[n][0]) for n in ("attn_q", "attn_k", "attn_v")}
+    q, att = new(heads * D), new(heads * D)
+    ones, hones = torch.ones(hid, device=dev), torch.ones(D, device=dev)
+    inv = (1e6 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)).float().to(dev)
+    row = -(-ctx // P)
+    table = torch.randperm(B * row, generator=g, device=dev).to(torch.int32).view(B, row)
+    lengths = torch.full((B,), ctx, dtype=torch.int32, device=dev)
+    batch = q4rdna.KVBatch(table, lengths, max_length=ctx)
+    # the cached tokens: the same random rows for every layer, appended as a prompt would be
+    part = min(ctx, 4096)
+    kv = torch.randn((2, part, kvh, D), generator=g, device=dev).to(torch.bfloat16)
+    plans, caches, wbytes = [], [], 0
+    for layer in range(per):
+        w = {}
+        for i, (n, (N, K)) in enumerate(shape.items()):
+            w[n] = synth.tiles_torch(N, K, args.seed + 1 + layer * len(shape) + i, dev)
+            wbytes += N * K * 34 // 64
+        plans.append((
+            q4rdna.Plan([{"tiles": w[n], "x": h, "y": qkv[n], "norm_weight": ones} for n in qkv], B=B),
+            q4rdna.Plan([{"tiles": w["attn_output"], "x": att, "y": mid, "op": q4rdna.OP_ADD, "add": h}], B=B),
+            q4rdna.Plan([{"tiles": w["ffn_up"], "gate_tiles": w["ffn_gate"], "x": mid, "y": act, "op": q4rdna.OP_SWIGLU,
+                          "norm_weight": ones}], B=B),
+            q4rdna.Plan([{"tiles": w["ffn_down"], "x": act, "y": h, "op": q4rdna.OP_ADD, "add": mid}], B=B)))
+        c = q4rdna.KVCache(B * row, P, kvh, D)
+        for s in range(B):
+            for at in range(0, ctx, part):
+                n = min(part, ctx - at)
+                one = q4rdna.KVBatch(table[s:s + 1], torch.tensor([at + n], dtype=torch.int32, device=dev),
+                                     q_start=torch.tensor([0, n], dtype=torch.int32, device=dev))
+                q4rdna.kv_append(c, one, kv[0, :n], kv[1, :n])
+        caches.append(c)
+    kvbytes = sum(c.tiles.numel() for c in caches)
+
+    def layers(products, attention):
+        for (pqkv, po, pglu, pdown), c in zip(plans, caches):
+            if products:
+                pqkv.run()
+            if attention:
+                q4rdna.kv_append(c, batch, qkv["attn_k"], qkv["attn_v"], q=qkv["attn_q"], q_out=q, inv_freq=inv,
+                                 q_norm=hones, k_norm=hones)
+                q4rdna.kv_attention(c, batch, q, out=att)
+            if products:
+                po.run()
+                pglu.run()
+                pdown.run()
+
+    def timed(products, attention):
+        def step():
+            h.copy_(x0)
+            layers(products, attention)
+
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        l0 = q4rdna.launch_count()
+        with torch.cuda.graph(graph):
+            step()
+        launches = q4rdna.launch_count() - l0
+        for _ in range(args.warmup):
+            graph.replay()
+        torch.cuda.synchronize()
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        for _ in range(args.steps):
+            graph.replay()
+        e1.record()
+        torch.cuda.synchronize()
+        return e0.elapsed_time(e1) * 1e3 / args.steps, launches
+
+    with ClockSampler(0) as clk:
+        us, launches = timed(True, True)
+    if q4rdna.take_fault() or not bool(torch.isfinite(h).all()):
+        raise SystemExit("the step failed")
+    prod, _ = timed(True, False)
+    attn, _ = timed(False, True)
+    total = wbytes + kvbytes
+    return {"metric": f"us per {args.model} decode step with attention over an int8 cache", "value": round(us, 2),
+            "unit": "us", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup, "ms_per_step": round(us / 1e3, 5),
+            "higher_is_better": False, "dtype": "int4 weights, int8 cache, f32 rows",
+            "data": "synthetic weights and cached tokens of the model's shapes",
+            "products_us": round(prod, 2), "append_attention_us": round(attn, 2),
+            "roofline": {"bytes": total, "gbs": round(total / us / 1e3, 1), "frac": round(total / us / 1e3 / peak, 4),
+                         "peak_gbs": peak, "peak": src,
+                         "append_attention_frac": round(kvbytes / attn / 1e3 / peak, 4)},
+            "config": {"workload": f"{per} layers, {B} sequences of {ctx} cached tokens", "batch": B, "tokens": ctx,
+                       "heads": heads, "kv_heads": kvh, "head_dim": D, "weight_bytes": wbytes, "cache_bytes": kvbytes,
+                       "l2": "no flush: every layer has its own weights and cache"},
+            "gpu_launches": launches * args.steps, "clocks": clk.summary()}
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -1001,6 +1125,9 @@ def main():
                     help="activation columns per GEMV (1..16; 3..16 run the tile path)")
     ap.add_argument("--hybrid", action="store_true",
                     help="the reference's qkv-fallback scope: attn_q/k/v as Q4_K tensors, the rest Q4_RDNA")
+    ap.add_argument("--attention", type=int, default=0, metavar="TOKENS",
+                    help="a whole decoder step with append and attention over a cache of TOKENS per sequence, "
+                         "--batch sequences")
     ap.add_argument("--single", action="store_true",
                     help="us per GEMV through the drop-in entry points (configs 0 and 1) instead of the step")
     ap.add_argument("--single-sweep", action="store_true", help="--single: also force split 1..16")
@@ -1029,6 +1156,8 @@ def main():
         out = run_pack(args)
     elif args.single:
         out = run_single(args)
+    elif args.attention:
+        out = run_attention(args)
     else:
         out = run_reference(args) if args.impl == "reference" else run_ours(args)
     if out is not None:
