@@ -104,14 +104,14 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    const long long left = find_share<kAttnWarps>(A, NC, 4, sm.share);
-    if (left == 0) {
+    const Share found = find_share<kAttnWarps>(A, NC, 4, sm.share);
+    if (found.left == 0) {
         if (threadIdx.x == 0) A.rec[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
         return;
     }
     bool open = false;  // the share ends inside a task that began in it
     const int t0 = 4 * (g >> 1) + (g & 1);  // K rows g and g + 8 of the fragments: tokens t0 and t0 + 2
-    Walk W(A, NC, 4, left, sm.share);
+    Walk W(A, NC, 4, found);
 
     uint4 kr[2][KW];
     uint32_t vr[4][VB / 4];

@@ -82,22 +82,52 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
     return a / b;
 }
 
-template <int WARPS>
-struct ShareSmem {
-    long long sum[WARPS];
-    long long rest;  // offset of the share's begin in sequence `seq`
-    long long share, head;  // head: the sequence's work per kv head
+// A CTA's share
+struct Share {
+    long long left;   // its length; 0: nothing
+    long long share;  // the length of every CTA's but the last
+    long long rest;   // offset of its begin in sequence `seq`
+    long long head;   // that sequence's work per kv head
     int seq;
     Seq q;
 };
-
-// Where the CTA's share begins: sequence and offset in its work (in sm); returns the
-// share's length (0: nothing).  All of the CTA's threads take part.
 template <int WARPS>
-__device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int shift, ShareSmem<WARPS> &sm) {
+struct ShareSmem {
+    long long sum[WARPS];
+    Share found;
+};
+
+// The CTA's share; all of its threads take part
+template <int WARPS>
+__device__ __forceinline__ Share find_share(const AttnArgs &A, int nc, int shift, ShareSmem<WARPS> &sm) {
     constexpr int THREADS = 32 * WARPS;
     const Batch &B = A.b;
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (B.S <= 32) {  // every warp by itself: no barrier
+        Seq q{0, 0, 0};
+        if (lane < B.S) q = load_seq(B, lane);
+        const long long head = head_work(A, q, nc, shift), mine = head * A.c.hk;
+        long long x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        const long long total = __shfl_sync(0xffffffffu, x, 31);
+        Share out{};
+        out.share = max((long long)A.min_share, quotient(total + gridDim.x - 1, gridDim.x));
+        const long long begin = out.share * blockIdx.x;
+        out.left = max(0LL, min(out.share, total - begin));
+        const unsigned behind = __ballot_sync(0xffffffffu, x > begin);
+        if (behind == 0) return out;
+        out.seq = __ffs(behind) - 1;
+        out.rest = begin - __shfl_sync(0xffffffffu, x - mine, out.seq);
+        out.head = __shfl_sync(0xffffffffu, head, out.seq);
+        out.q.a = __shfl_sync(0xffffffffu, q.a, out.seq);
+        out.q.n = __shfl_sync(0xffffffffu, q.n, out.seq);
+        out.q.L = __shfl_sync(0xffffffffu, q.L, out.seq);
+        return out;
+    }
     Seq q{0, 0, 0};
     auto work = [&](int s) -> long long {
         q = Seq{0, 0, 0};
@@ -120,8 +150,7 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
     }
     const long long share = max((long long)A.min_share, quotient(total + gridDim.x - 1, gridDim.x));
     const long long begin = share * blockIdx.x;
-    if (begin >= total) return 0;
-    if (threadIdx.x == 0) sm.share = share;
+    if (begin >= total) return Share{};
     long long before = 0;
     for (int base = 0; base < B.S && before <= begin; base += THREADS) {
         const long long mine = base == 0 && B.S <= THREADS ? first : work(base + threadIdx.x);  // (and q)
@@ -142,15 +171,12 @@ __device__ __forceinline__ long long find_share(const AttnArgs &A, int nc, int s
         x += ahead;
         const long long at = begin - before - (x - mine);
         if (at >= 0 && at < mine) {
-            sm.seq = base + threadIdx.x;
-            sm.rest = at;
-            sm.q = q;
-            sm.head = quotient(mine, A.c.hk);
+            sm.found = {min(share, total - begin), share, at, quotient(mine, A.c.hk), base + (int)threadIdx.x, q};
         }
         before += all;
         __syncthreads();
     }
-    return min(share, total - begin);
+    return sm.found;
 }
 
 // The tasks of a share, one after the other (the same in all threads; the lanes of a
@@ -167,12 +193,11 @@ struct Walk {
     int begin = 0, end = 0, all = 0, cnt = 0;
     bool begins = false, ends = false;
 
-    template <class Smem>
-    __device__ __forceinline__ Walk(const AttnArgs &a, int nc_, int shift_, long long left_, const Smem &sm)
-        : A(a), nc(nc_), shift(shift_), left(left_), rest(sm.rest), share(sm.share), s(sm.seq), q(sm.q) {
+    __device__ __forceinline__ Walk(const AttnArgs &a, int nc_, int shift_, const Share &f)
+        : A(a), nc(nc_), shift(shift_), left(f.left), rest(f.rest), share(f.share), s(f.seq), q(f.q) {
         cols = q.n * A.group;
-        h = (int)quotient(rest, sm.head);
-        rest -= h * sm.head;
+        h = (int)quotient(rest, f.head);
+        rest -= h * f.head;
         col0 = -nc;
     }
 
@@ -276,8 +301,10 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
 }
 
 // Joins the pieces of the task that began in CTA blockIdx.x's share and went on in the
-// next ones: bound by the latency of a few dependent loads, so as many as can be are on
-// their way together.
+// next ones: bound by the latency of a few dependent loads (about 3.6 us behind the
+// attention), so as many as can be are on their way together.  One CTA per share and
+// column: a grid of as many CTAs as there can be tasks, each looking for its record
+// among all shares', took 1.8 us more for 8 tasks in 296 shares.
 
 constexpr int kJoinWarps = 8;
 

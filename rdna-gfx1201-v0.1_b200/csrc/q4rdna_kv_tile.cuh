@@ -627,10 +627,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    const long long left = find_share<kTileWarps>(A, kTileCols, kTileShift, sm.share);
+    const Share found = find_share<kTileWarps>(A, kTileCols, kTileShift, sm.share);
     bool ok = true, open = false;
-    if (left > 0) {
-        Walk W(A, kTileCols, kTileShift, left, sm.share);
+    if (found.left > 0) {
+        Walk W(A, kTileCols, kTileShift, found);
         uint32_t it = 0;   // steps so far: stage it % 2
         uint32_t st[2] = {0, 0}, tt[2] = {0, 0};  // steps of either tile, and tasks with steps
         while (W.next()) {
@@ -1022,10 +1022,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile32_kernel(const __grid
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    const long long left = find_share<kTileWarps>(A, kTile32Cols, kTileShift, sm.share);
+    const Share found = find_share<kTileWarps>(A, kTile32Cols, kTileShift, sm.share);
     bool ok = true, open = false;
-    if (left > 0) {
-        Walk W(A, kTile32Cols, kTileShift, left, sm.share);
+    if (found.left > 0) {
+        Walk W(A, kTile32Cols, kTileShift, found);
         uint32_t it = 0, task = 0;  // steps and tasks with steps so far
         while (W.next()) {
             const Seq &sq = W.q;
