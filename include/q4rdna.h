@@ -407,7 +407,7 @@ typedef struct q4rdna_kv_attention_args {
     int tokens; /* rows of q and out */
     int heads;  /* query heads, a multiple of kv_heads; head h reads kv head h * kv_heads / heads */
     const void *q;
-    void *out;
+    void *out; /* may be q itself */
     int64_t q_stride, out_stride;
     float scale; /* of q . k; 0: 1 / sqrt(head_dim) */
     int window;  /* a token sees itself and the window - 1 tokens before it; 0: all of them */
@@ -427,7 +427,8 @@ size_t q4rdna_kv_cache_bytes(const q4rdna_kv_cache *cache);
  * held tokens of this sequence (its first row is older than this call) and 0
  * otherwise.  Where s grew, the older codes become round(code * s_before / s);
  * the new ones are round(x / s), to nearest even.  Rows of a tile behind the
- * last token keep their bytes.  A k or v that is not finite makes its tile's
+ * last token keep their bytes, rows of q_out outside every sequence their values.
+ * A k or v that is not finite makes its tile's
  * scale NaN (so that every row that sees the tile becomes NaN) until the tile
  * is begun anew.  Two sequences of one call must not write the same tile. */
 q4rdna_status q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,

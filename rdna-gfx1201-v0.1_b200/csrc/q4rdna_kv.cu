@@ -40,7 +40,8 @@ q4rdna_status check_cache(const q4rdna_kv_cache *c, Cache &out) {
 }
 
 q4rdna_status check_batch(const q4rdna_kv_cache *c, const q4rdna_kv_batch *b, int tokens, Batch &out) {
-    if (b == nullptr || b->page_table == nullptr || b->lengths == nullptr) return Q4RDNA_ERR_INVALID_ARGUMENT;
+    if (b == nullptr) return Q4RDNA_ERR_INVALID_ARGUMENT;
+    if (b->sequences != 0 && (b->page_table == nullptr || b->lengths == nullptr)) return Q4RDNA_ERR_INVALID_ARGUMENT;
     if (b->sequences < 0 || b->table_stride <= 0 || b->max_length < 0 || tokens < 0) return Q4RDNA_ERR_INVALID_ARGUMENT;
     if (b->q_start == nullptr && tokens != b->sequences) return Q4RDNA_ERR_SHAPE;
     const long long room = std::min<long long>((long long)b->table_stride * c->page_tokens, 1 << 30);
@@ -148,7 +149,7 @@ AppendVariant append_variant(int type, int format, int turn) {
 }
 
 // Raises a kernel's shared-memory limit, once per device
-bool raise_smem(const void *kernel, int bytes) {
+bool raise_smem(const void *kernel, int bytes) try {
     static std::mutex mu;
     static std::set<std::pair<int, const void *>> done;
     int dev = 0;
@@ -161,6 +162,8 @@ bool raise_smem(const void *kernel, int bytes) {
     }
     done.insert({dev, kernel});
     return true;
+} catch (...) {  // out of memory: nothing may be thrown through the C functions
+    return false;
 }
 
 // ---- the attention's launches
@@ -207,7 +210,7 @@ struct AttnLaunch {
 };
 
 // CTAs of the kernel that the current device holds at once (its shared-memory limit raised); 0 on an error
-int resident_ctas(const Variant &v) {
+int resident_ctas(const Variant &v) try {
     static std::mutex mu;
     static std::map<std::pair<int, AttnKernel>, int> known;
     int dev = 0;
@@ -225,6 +228,8 @@ int resident_ctas(const Variant &v) {
         n = sms * std::max(occ, 1);
     }
     return n;
+} catch (...) {
+    return 0;
 }
 
 q4rdna_status size_launch(const AttnArgs &A, int D, AttnLaunch &L) {

@@ -14,7 +14,8 @@
 //     heads run side by side.
 //   * Cosines and sines are made once per CTA, in shared memory and the lanes' order:
 //     position * inv_freq and the reduction to a turn in f64 (an f32
-//     product is off by 0.06 rad at position 10^6), then sincospif of the f32 rest.
+//     product is off by 0.06 rad at position 10^6), then sincospif of the f32 rest
+//     and what its rounding lost (2^-24 of the angle) to first order.
 //   * A lane's rows come through a ring in shared memory, 6 (f32: 4) ahead, from before
 //     the cosines on.
 //   * Keys and values stay in registers between the maximum and the codes.  A code is
@@ -245,7 +246,12 @@ __global__ void __launch_bounds__(D, 640 / D) kv_append_kernel(const __grid_cons
         if (p < half) {
             const int pos = A.positions != nullptr ? A.positions[row0 + t] : lo + t;
             const double a = (double)pos * (double)A.inv_freq[p] * 0.3183098861837907;  // in half turns
-            sincospif((float)(a - 2.0 * rint(0.5 * a)), &sn, &c);
+            const double turn = a - 2.0 * rint(0.5 * a);
+            const float f = (float)turn, d = 3.14159265f * (float)(turn - f);  // what f lost, to first order
+            float s0, c0;
+            sincospif(f, &s0, &c0);
+            sn = fmaf(d, c0, s0);
+            c = fmaf(-d, s0, c0);
         }
         // pair p is the e-th of lane x
         const int x = P::lane(TURN != kTurnPairs ? p : 2 * p), e = TURN != kTurnPairs ? P::slot(p) : P::slot(2 * p) / 2;
@@ -268,7 +274,9 @@ __global__ void __launch_bounds__(D, 640 / D) kv_append_kernel(const __grid_cons
 #pragma unroll
             for (int i = 1; i < 8; ++i) ss = fma2(x[i], x[i], ss);
             const float2 two = both(ss);
-            const float f1 = rsqrtf(group_sum<LPR>(two.x + two.y) * (1.0f / D) + A.eps);
+            const float ms = group_sum<LPR>(two.x + two.y) * (1.0f / D) + A.eps;
+            float f1 = rsqrtf(ms);
+            if (ms > 0.0f && f1 > 0.0f) f1 = fmaf(0.5f * f1, fmaf(-ms * f1, f1, 1.0f), f1);  // Newton: rsqrtf is off by 2 ulp
             const F2 f = pack2(f1, f1);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

@@ -6,6 +6,7 @@
 // stream, and allocates there.  Argument errors raise ValueError; a status of the
 // library goes to the package's check(), which raises its own error.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -43,7 +44,10 @@ struct Raised {};  // a Python error is set
 
 const at::Tensor &tensor(PyObject *o, const char *name) {
     if (!THPVariable_Check(o)) throw Refused(std::string("kv cache operators: ") + name + " is a tensor");
-    return THPVariable_Unpack(o);
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (t.requires_grad() && c10::GradMode::is_enabled())
+        throw Refused(std::string("kv cache operators have no gradients: ") + name + " requires one (not under torch.no_grad())");
+    return t;
 }
 bool given(PyObject *o) { return o != Py_None; }
 

@@ -570,8 +570,9 @@ def kv_append(cache: KVCache, batch: KVBatch, k, v, *, q=None, q_out=None, inv_f
     k, v [rows, kv_heads, head_dim] and q [rows, heads, head_dim] (f32, f16 or
     bf16; rows may be strided).  q_norm / k_norm (f32 [head_dim]) apply the
     per-head RMSNorm; inv_freq (f32 [rotary_dim / 2]) the rotation at positions
-    (int32 [rows]; None: the token's number).  Returns the rotated q (q_out, or a
-    new tensor), None without q.
+    (int32 [rows]; None: the token's number).  Returns the rotated q (q_out, which
+    may be q itself, or a new tensor, whose rows outside every sequence are
+    undefined), None without q.  No gradients.
     """
     f = (_kv_module or _kv()).append
     a = (cache._at, batch._at, k, v, q, q_out, inv_freq, rotary_dim, rope, positions, q_norm, k_norm, norm_eps)
@@ -582,7 +583,8 @@ def kv_attention(cache: KVCache, batch: KVBatch, q, *, scale: float = 0.0, windo
     """softmax(scale * q k^T) v over the cache (q4rdna_kv_attention): each row of
     q [rows, heads, head_dim] sees its sequence's tokens up to itself, at most
     `window` of them (0: all).  scale 0: 1 / sqrt(head_dim).  A row that sees
-    nothing becomes 0; rows outside every sequence are left as they were."""
+    nothing becomes 0; rows of out (which may be q itself) outside every sequence
+    are left as they were, undefined in a new tensor.  No gradients."""
     f = (_kv_module or _kv()).attention
     if stream is None:
         return f(cache._at, batch._at, q, scale, window, out)

@@ -184,3 +184,22 @@ def test_columns_past_32_bits_are_refused():
     args = dict(tokens=n, heads=h, q_stride=h * 128, out_stride=h * 128)
     assert q4rdna.lib.q4rdna_kv_attention(c, b, *refs(attention_args(**args)), A, 1 << 40, None) == TOO_LARGE
     assert q4rdna.lib.q4rdna_kv_attention_workspace_bytes(c, b, *refs(attention_args(**args))) == 0
+
+
+def test_an_empty_batch_needs_no_arrays():
+    c, b = refs(desc(), batch(page_table=None, lengths=None, sequences=0))
+    assert q4rdna.lib.q4rdna_kv_append(c, b, *refs(append_args(tokens=0, k=None, v=None, q=None, q_out=None)), None) == 0
+    assert q4rdna.lib.q4rdna_kv_attention(c, b, *refs(attention_args(tokens=0, q=None, out=None)), None, 0, None) == 0
+
+
+def test_gradients_are_refused():
+    """No operator of the cache has a backward pass: a graph that needs one is not cut silently."""
+    cache = q4rdna.KVCache(4, 16, 2, 64, device="cpu")
+    batch = q4rdna.KVBatch(torch.zeros((3, 2), dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+    x, leaf = torch.zeros((3, 2, 64)), torch.zeros((3, 2, 64), requires_grad=True)
+    for call in (lambda: q4rdna.kv_attention(cache, batch, leaf), lambda: q4rdna.kv_append(cache, batch, leaf, x),
+                 lambda: q4rdna.kv_append(cache, batch, x, leaf)):
+        with pytest.raises(ValueError, match="no gradients"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA tensor"):  # goes on to the next check
+            call()

@@ -105,6 +105,37 @@ def test_attention_many_sequences(cuda):
     attend(cuda, 810, lengths, [1] * 700, 1, 2, 64, 16, KV_INT8, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S", [31, 32, 33, 64, 65])
+def test_attention_batches_about_a_warp(cuda, S, dtype):
+    """Sequences of no, one, some and many new tokens side by side."""
+    g = torch.Generator().manual_seed(S)
+    lengths = torch.randint(40, 300, (S,), generator=g).tolist()
+    news = [(1, 0, 3, 40, 1, 1, 2, 1)[(s * 5 + s // 8) % 8] for s in range(S)]
+    attend(cuda, 815 + S, lengths, news, 2, 4, 64, 16, KV_INT8, dtype)
+    attend(cuda, 817 + S, lengths, [1] * S, 2, 4, 128, 16, KV_E4M3, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lengths,news", [([7001, 60], [1, 1]), ([4000, 33, 500], [3, 33, 200]), ([2500], [700])])
+def test_attention_in_place(cuda, lengths, news, dtype):
+    cache, _, table = make(cuda, 825, lengths, 2, 128, 32, KV_INT8)
+    start = i32([sum(news[:s]) for s in range(len(news) + 1)], cuda)
+    batch = KVBatch(table.to(cuda), i32(lengths, cuda), q_start=None if news == [1, 1] else start)
+    q = torch.randn((sum(news), 8, 128), device=cuda).to(dtype)
+    want = q4rdna.kv_attention(cache, batch, q)
+    got = q4rdna.kv_attention(cache, batch, q, out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(q, want)
+
+
+def test_empty_batch(cuda):
+    cache = KVCache(2, 16, 2, 64)
+    batch = KVBatch(torch.zeros((0, 3), dtype=torch.int32, device=cuda), i32([], cuda))
+    x = torch.zeros((0, 2, 64), device=cuda)
+    assert q4rdna.kv_append(cache, batch, x, x, q=x).shape == x.shape
+    assert q4rdna.kv_attention(cache, batch, x).shape == x.shape
+
+
 def test_attention_scores_far_apart(cuda):
     """Scores of hundreds: one token takes all the weight; and a scale of its own."""
     attend(cuda, 820, [333], [1], 2, 4, 128, 16, KV_INT8, torch.float32, q_scale=60.0)
