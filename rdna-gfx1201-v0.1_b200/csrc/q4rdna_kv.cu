@@ -260,8 +260,12 @@ q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &
     // (one sequence, or a few of many columns on average: no launch for the others, which the tile kernels take too)
     const bool alone = A.b.S == 1 || A.b.q_start == nullptr || (A.b.S <= 4 && most >= 4LL * kTileFrom * A.b.S);
     if (!tiles || !alone) {
-        // one column tile where a token's heads fit it and each sequence has one token, else two
-        const int nt = A.b.q_start == nullptr && A.group <= 8 ? 1 : 2, terms = A.type == Q4RDNA_F32 ? 2 : 1;
+        // One column tile (two CTAs an SM; a sequence of more columns has several tasks) or two, us for 16 sequences of
+        // 4001 tokens, 8 kv heads, f32:
+        //   columns             8       16       32
+        //   head_dim 128   37, 50   55, 56   74, 79
+        //   head_dim 256   56, 83   92, 99  131, 139   (4 kv heads, 9664 columns, 604 tokens: 954, 831)
+        const int nt = (long long)A.b.T * A.group <= 32LL * A.b.S ? 1 : 2, terms = A.type == Q4RDNA_F32 ? 2 : 1;
         AttnLaunch &l = L[n++];
         l.v = D == 64 ? variant<64>(A.c.format, nt, terms)
                       : D == 128 ? variant<128>(A.c.format, nt, terms) : variant<256>(A.c.format, nt, terms);
