@@ -20,6 +20,13 @@
 //     the output dims is as good as another, so the order is chosen such that a lane
 //     loads 16 bytes at a time: K, dims 16 c .. 16 c + 15 of tokens t0 and t0 + 2; V,
 //     dims D/8 g .. of tokens 4 c .. 4 c + 3 (lane = 4 g + c).
+//
+// Measured (8 kv heads of 128, device time with the join): 128 sequences of up to 4093
+// tokens, 64 query heads, e4m3, bf16 143 us, 0.62 of the bytes' time at 6543 GB/s; 32
+// query heads, int8, f32: 16 sequences of up to 8191 48 us and one of 65521 41 us, both
+// 0.50, one of 517 12 us.  About 17 us of a call are fixed: the table of shares, the
+// latency of the first loads, the meeting of the warps, the join.  Sums by int8 products
+// (codes as they are, q in digits) took 164 us where this took 157 (64 of 8191).
 #pragma once
 
 #include "q4rdna_kv_split.cuh"

@@ -21,6 +21,12 @@
 //     weights would leave f16's range (the row's O is then rescaled by its own thread),
 //     and p carries 2^7.
 //   * Tensor memory (512 columns): S0 S1 O0 O1, 128 each.
+// Measured (device time with the join): 2048 tokens behind 8191 others, 32 query and 8 kv
+// heads of 128, e4m3, bf16 425 us, 0.44 of the products' time at 1650 TFLOP/s; three
+// prompts of up to 1900, 16 and 4 heads of 64, window 1000, f16 91 us.  Work left out in turn, when the first took 460 us: 354 without
+// the loading warps' conversion, 308 without the exponentials too, 300 with the products
+// and the waits alone.  So no unit is full: what bounds it are the waits between the
+// roles, the softmax's latency (about 3000 cycles a tile and step) above all.
 // Every wait is bounded (about a second, %globaltimer): on expiry the role sets bit 4
 // of the fault word and takes no more waits, copies or products; the issuing thread
 // still waits (bounded) for its products before the tensor memory is freed.
@@ -782,6 +788,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
 // a task's products would cost 2^-17.  A task is 128 columns, one tile; Q's two terms
 // take the two Q buffers, S two buffers in turn (the next step's S is made under this
 // step's softmax), then the step's O and the task's O.  Warps 4-7 add one to the other.
+// 1024 tokens behind 1024 others, 32 and 8 heads of 128: 143 us (bf16 rows 100 us).
 
 constexpr int kTile32Cols = 128;
 
