@@ -22,9 +22,9 @@
 //     dims D/8 g .. of tokens 4 c .. 4 c + 3 (lane = 4 g + c).
 //
 // Measured (8 kv heads of 128, device time with the join): 128 sequences of up to 4093
-// tokens, 64 query heads, e4m3, bf16 143 us, 0.62 of the bytes' time at 6543 GB/s; 32
-// query heads, int8, f32: 16 sequences of up to 8191 48 us and one of 65521 41 us, both
-// 0.50, one of 517 12 us.  About 17 us of a call are fixed: the table of shares, the
+// tokens, 64 query heads, e4m3, bf16 140 us, 0.64 of the bytes' time at 6543 GB/s; 32
+// query heads, int8, f32: 16 sequences of up to 8191 47 us and one of 65521 40 us, both
+// 0.51, one of 517 12 us.  About 17 us of a call are fixed: the table of shares, the
 // latency of the first loads, the meeting of the warps, the join.  Sums by int8 products
 // (codes as they are, q in digits) took 164 us where this took 157 (64 of 8191).
 #pragma once
@@ -252,6 +252,11 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
             b += kAttnWarps;
             ++at;
             const uint8_t *next = next_tile();
+            // its registers are free only as this block's are used up; until then it comes to L2 (128 x 4093: 143 -> 140
+            // us; the block after it too: 148)
+            if (next != nullptr)
+                for (int i = lane * 128; i < kHeader + 2 * kBlock * D; i += 32 * 128)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(next + i) : "memory");
 
             // scores
             float sa[NT][TERMS][4];
