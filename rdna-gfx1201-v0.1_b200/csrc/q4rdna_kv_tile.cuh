@@ -628,10 +628,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Bars bar{smem_u32(sm.bar)};
 
-    const uint32_t tmem = tile_enter<D>(sm, bar);
-    // only now: a dependent kernel that takes tensor memory must not come before this CTA
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // Tensor memory is taken between the two: behind every kernel of the stream before this one, which may still
+    // want some of its own (this CTA would hold it and wait for that kernel), and before every one after it
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t tmem = tile_enter<D>(sm, bar);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const Share found = find_share<kTileWarps>(A, kTileCols, kTileShift, sm.share);
     bool ok = true, open = false;
@@ -1024,10 +1025,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile32_kernel(const __grid
     Smem &sm = *reinterpret_cast<Smem *>(tile_smem);
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Bars bar{smem_u32(sm.bar)};
-    const uint32_t tmem = tile_enter<D>(sm, bar);
-    // only now: a dependent kernel that takes tensor memory must not come before this CTA
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // Tensor memory is taken between the two: behind every kernel of the stream before this one, which may still
+    // want some of its own (this CTA would hold it and wait for that kernel), and before every one after it
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t tmem = tile_enter<D>(sm, bar);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const Share found = find_share<kTileWarps>(A, kTile32Cols, kTileShift, sm.share);
     bool ok = true, open = false;

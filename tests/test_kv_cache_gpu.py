@@ -431,6 +431,36 @@ def test_dequant(cuda, D, P, fmt, dtype):
 
 # ------------------------------------------------- streams, graphs, the chain
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompt_attention_between_products_of_16_columns(cuda, dtype):
+    """Kernels with tensor memory of their own on both sides, each one set up while the one before it ends."""
+    H, G, D, n = 2, 8, 64, 16
+    cache, tiles, table = make(cuda, 1150, [900], H, D, 32, KV_INT8)
+    batch = KVBatch(table.to(cuda), i32([900], cuda), q_start=i32([0, n], cuda))
+    w = torch.from_numpy(synth.tiles_np(H * G * D, 512, 9)).to(cuda)
+    x = torch.randn((n, 512), device=cuda)
+    y, z = torch.zeros((n, H * G * D), device=cuda), torch.zeros((n, H * G * D), device=cuda)
+    first, last = q4rdna.Plan([{"tiles": w, "x": x, "y": y}], B=n), q4rdna.Plan([{"tiles": w, "x": x, "y": z}], B=n)
+    rows = torch.randn((n, H * G, D), device=cuda).to(dtype)
+
+    def chain():
+        for _ in range(20):
+            first.run()
+            out = q4rdna.kv_attention(cache, batch, rows)
+            last.run()
+        return out
+
+    chain()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = chain()
+    for _ in range(5):
+        g.replay()
+    torch.cuda.synchronize()
+    assert q4rdna.take_fault() == 0 and torch.equal(y, z)
+    ref.check_attention(out, ref.attention(tiles, D, KV_INT8, table, [900], [n], rows.cpu()), dtype)
+
 def test_side_stream_and_graphs(cuda):
     """Two captured calls replayed on two streams at once, lengths changed between
     replays; and a call on a stream that is not current."""
@@ -547,3 +577,21 @@ def test_decoder_attention_block(cuda, tokens):
         o = a @ W["o"].T + h.double().cpu()
         assert ((out.double().cpu() - o).abs() <= 1e-5 * (a.abs() @ W["o"].abs().T + h.abs().cpu())).all()
     assert q4rdna.take_fault() == 0
+
+
+@pytest.mark.parametrize("model,batch", [("qwen3-8b", 1), ("qwen3-32b", 9)])
+def test_bench_runs_a_decoder_step(cuda, model, batch):
+    """bench.py --attention: one layer, a cache whose last page is not full."""
+    import json
+    import os
+    import subprocess
+    import sys
+
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, os.path.join(repo, "bench.py"), "--attention", "203", "--layers", "1", "--model",
+                        model, "--batch", str(batch), "--steps", "3", "--warmup", "3"], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    out = json.loads(r.stdout)
+    assert out["config"]["kv_heads"] == 8 and out["config"]["heads"] == (32 if model == "qwen3-8b" else 64)
+    assert out["gpu_launches"] > 0 and 0 < out["append_attention_us"] < out["value"] < 1e5
