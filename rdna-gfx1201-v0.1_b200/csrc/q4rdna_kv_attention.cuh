@@ -40,16 +40,19 @@ constexpr float kStep = 8.0f;   // m moves when a score outgrows it by more
 
 // ------------------------------------------------------------ fragments
 
+// Ordinary loads: the kernel is resident while the append before it in the stream writes these tiles, and the
+// read-only path promises data that nobody writes as long as the kernel lives (griddepcontrol.wait makes the
+// writes visible to ordinary loads; the times are the same)
 __device__ __forceinline__ uint4 ld_stream(const uint8_t *p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "l"(p));
     return v;
 }
 __device__ __forceinline__ uint2 ld_stream2(const uint8_t *p) {
     uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
     return v;
 }
 
@@ -176,7 +179,7 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
         if (tile != nullptr) {
             load_k(tile);
             load_v(tile);
-            sc = __ldg(reinterpret_cast<const float2 *>(tile));
+            sc = *reinterpret_cast<const float2 *>(tile);
         }
     };
     bool more = W.next();
@@ -296,7 +299,7 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
             const float2 scale = sc;
             if (next != nullptr) {
                 load_k(next);
-                sc = __ldg(reinterpret_cast<const float2 *>(next));
+                sc = *reinterpret_cast<const float2 *>(next);
             }
 
             // softmax weights; lane: tokens t0, t0 + 2 of columns 2 c, 2 c + 1

@@ -203,3 +203,17 @@ def test_gradients_are_refused():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA tensor"):  # goes on to the next check
             call()
+
+
+def test_tiles_are_read_by_ordinary_loads():
+    """The attention is resident while the append before it writes the tiles: nothing is read as data that
+    no one writes during the kernel."""
+    import os
+
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rdna-gfx1201-v0.1_b200", "csrc")
+    names = [n for n in os.listdir(csrc) if n.startswith("q4rdna_kv")]
+    assert len(names) >= 7
+    for n in names:
+        with open(os.path.join(csrc, n)) as f:
+            text = f.read()
+        assert "ld.global.nc" not in text and "__ldg" not in text, n

@@ -461,6 +461,34 @@ def test_prompt_attention_between_products_of_16_columns(cuda, dtype):
     assert q4rdna.take_fault() == 0 and torch.equal(y, z)
     ref.check_attention(out, ref.attention(tiles, D, KV_INT8, table, [900], [n], rows.cpu()), dtype)
 
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fmt", [KV_INT8, KV_E4M3])
+@pytest.mark.parametrize("n", [1, 24])
+def test_attention_directly_behind_appends(cuda, n, fmt, dtype):
+    """Steps of one token (and of 24: the kernel for many columns) over pages of 16, nothing awaited between append
+    and attention: the step that fills a tile's slot 15, whose bytes share a sector with the next head's scales,
+    and the one that begins the next tile are checked on the cache as it stood."""
+    H, G, D, P, steps = 8, 4, 128, 16, 49 if n == 1 else 8
+    cache, _, table = make(cuda, 1160, [n * steps] * 2, H, D, P, fmt)
+    g = torch.Generator().manual_seed(7)
+    dev = table.to(cuda)
+    start = i32([0, n, 2 * n], cuda)
+    rows = [[torch.randn((2 * n, h, D), generator=g).to(dtype).to(cuda) for h in (H, H, H * G)] for _ in range(steps)]
+    batches = [KVBatch(dev, i32([n * i, n * i], cuda), q_start=start) for i in range(1, steps + 1)]
+    kept = []
+    torch.cuda.synchronize()
+    for i, ((k, v, q), batch) in enumerate(zip(rows, batches), 1):
+        q4rdna.kv_append(cache, batch, k, v)
+        out = q4rdna.kv_attention(cache, batch, q)
+        if n > 1 or i % 16 < 2:
+            kept.append((i, q, out, cache.tiles.clone()))
+    for i, q, out, tiles in kept:
+        want = ref.attention(tiles.cpu(), D, fmt, table, [n * i] * 2, [n, n], q.cpu())
+        ref.check_attention(out, want, dtype, f"step {i}")
+    assert q4rdna.take_fault() == 0
+
+
 def test_side_stream_and_graphs(cuda):
     """Two captured calls replayed on two streams at once, lengths changed between
     replays; and a call on a stream that is not current."""
