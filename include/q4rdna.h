@@ -429,8 +429,8 @@ size_t q4rdna_kv_cache_bytes(const q4rdna_kv_cache *cache);
  * the new ones are round(x / s), to nearest even.  Rows of a tile behind the
  * last token keep their bytes, rows of q_out outside every sequence their values.
  * A k or v that is not finite makes its tile's
- * scale NaN (so that every row that sees the tile becomes NaN) until the tile
- * is begun anew.  Two sequences of one call must not write the same tile. */
+ * scale NaN (so that every row that sees the tile becomes NaN) and its new codes
+ * 0 (so that no other row does) until the tile is begun anew.  Two sequences of one call must not write the same tile. */
 q4rdna_status q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
                                const q4rdna_kv_append_args *args, q4rdna_stream_t stream);
 

@@ -407,6 +407,8 @@ __global__ void __launch_bounds__(D, 640 / D) kv_append_kernel(const __grid_cons
                     }
                 if (here && on) {
                     codes_of<FMT>(k, hi, low, c);
+                    // the scale marks the tile; a NaN code would reach rows that do not see it, as 0 * NaN
+                    if (isnan(x)) c[0] = c[1] = make_uint2(0, 0);
                     put_codes(codes + (r0 + tok) * D, c);
                 }
                 if (here && tok == 0 && l == 0) reinterpret_cast<float *>(tile)[y] = x;

@@ -389,6 +389,44 @@ def test_append_not_finite(cuda):
         assert not torch.isnan(sb).any()
 
 
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("fmt", [KV_INT8, KV_E4M3])
+def test_append_not_finite_spoils_only_rows_that_see_it(cuda, fmt, bad, which):
+    """A NaN or infinity is appended, then attended over: rows behind it in the causal order, or with a window that has
+    passed its tile, are as without it; rows that see the tile are NaN.  Few and many columns, with and without a window."""
+    H, G, D, P, L, at = 2, 4, 64, 16, 300, 70  # token 70: tile 64..79
+    clean, tiles, table = make(cuda, 985, [L], H, D, P, fmt)
+    dirty = KVCache(tiles.shape[0], P, H, D, format=fmt, tiles=tiles.to(cuda))
+    g = torch.Generator().manual_seed(9)
+    rows = {n: torch.randn((L, H, D), generator=g).to(cuda) for n in "kv"}
+    whole = KVBatch(table.to(cuda), i32([L], cuda), q_start=i32([0, L], cuda))
+    q4rdna.kv_append(clean, whole, rows["k"], rows["v"])
+    rows[which] = rows[which].clone()
+    rows[which][at, 1, 5] = bad
+    q4rdna.kv_append(dirty, whole, rows["k"], rows["v"])
+    for n in (1, 3, 40, 280):
+        for last in (L, 100, 82, 66):
+            if n > last:
+                continue
+            batch = KVBatch(table.to(cuda), i32([last], cuda), q_start=i32([0, n], cuda))
+            q = torch.randn((n, H * G, D), generator=g).to(cuda)
+            for dtype in (torch.float32, torch.bfloat16):
+                for window in (0, 10):
+                    a, b = (q4rdna.kv_attention(c, batch, q.to(dtype), window=window) for c in (clean, dirty))
+                    tok = torch.arange(last - n, last, device=cuda)
+                    sees = (tok >= 64) & ((tok - (window or L + 1) + 1) <= 79)
+                    hit = torch.zeros((n, H * G), dtype=torch.bool, device=cuda)
+                    hit[:, G:] = sees[:, None]
+                    assert torch.equal(b[~hit], a[~hit]) and torch.isfinite(a).all(), (n, last, dtype, window)
+                    assert torch.isnan(b[hit]).all(), (n, last, dtype, window)
+    # one token more in the spoilt tile, and the tile begun anew
+    batch = KVBatch(table.to(cuda), i32([72], cuda))
+    q4rdna.kv_append(dirty, batch, rows["k"][:1], rows["v"][:1])
+    for c in ref.parts(dirty.tiles, D, fmt)[1:]:
+        assert torch.isfinite(c.float()).all()
+
+
 def test_append_tiny_values(cuda):
     """Values whose scale would fall under 2^-100 are stored as zeros, scale 0."""
     H, D = 1, 64
