@@ -441,7 +441,9 @@ q4rdna_status q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_bat
  * f32), 16-bit rows with weights in f16; results do not depend on the timing.
  * The workspace (q4rdna_kv_attention_workspace_bytes, 16-byte aligned)
  * needs no initialisation and carries nothing from call to call; calls that
- * may overlap on the GPU need one each. */
+ * may overlap on the GPU need one each.  Tokens on a page outside the cache are
+ * not seen; a sequence with a length outside [0, max_length] has no tokens; each
+ * sets bit 3 of q4rdna_take_fault. */
 q4rdna_status q4rdna_kv_attention(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
                                   const q4rdna_kv_attention_args *args, void *workspace, size_t workspace_bytes,
                                   q4rdna_stream_t stream);

@@ -440,7 +440,9 @@ __device__ __noinline__ bool load_steps(const AttnArgs &A, const LoadPlace &plac
             if (z == 0 && u < 32) {
                 if (u < 8) {
                     const float sv = head.y <= kTinyScale ? kTinyScale : head.y;  // NaN stays
-                    P.scale[n & 3][u] = make_float4(head.x, log2f(sv), 1.0f / sv, 0.0f);
+                    // a block on a page outside the cache takes no weight, as if it were masked
+                    P.scale[n & 3][u] =
+                        tile0 != 0 ? make_float4(head.x, log2f(sv), 1.0f / sv, 0.0f) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
                 }
                 __syncwarp();
                 if (lane == 0) bar_arrive(P.sc_full + 8 * (n & 3));

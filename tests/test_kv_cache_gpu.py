@@ -261,6 +261,37 @@ def test_bad_metadata_sets_the_fault(cuda):
     assert not kk[:2].any() and not vv[:2].any() and kk[2].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [2, 45])
+def test_attention_without_a_page(cuda, n, D, dtype):
+    """Tokens on a page outside the cache are not seen, whichever kernel the columns choose; the other sequence is right."""
+    H, G, P, L = 2, 4, 32, 200
+    cache, tiles, table = make(cuda, 885, [L, L], H, D, P, KV_INT8)
+    q = torch.randn((2 * n, H * G, D), generator=torch.Generator().manual_seed(1)).to(dtype)
+    start = i32([0, n, 2 * n], cuda)
+    for missing in ([2], [0, 1, 2, 3], [4, 6], list(range(7))):
+        bad = table.clone()
+        bad[1, missing] = torch.tensor([tiles.shape[0], -1, 2 ** 31 - 1] * 3)[: len(missing)].int()
+        batch = KVBatch(bad.to(cuda), i32([L, L], cuda), q_start=start)
+        out = q4rdna.kv_attention(cache, batch, q.to(cuda))
+        assert q4rdna.take_fault() == 8
+        ref.check_attention(out[:n], ref.attention(tiles, D, KV_INT8, table, [L], [n], q[:n]), dtype, "other sequence")
+        kk, vv = (x[table[1, :7].long()].transpose(0, 1).flatten(1, 2)[:, :L] for x in ref.numbers(tiles, D, KV_INT8))
+        there = torch.tensor([t // P not in missing for t in range(L)])
+        want = [torch.zeros((n, H * G, D), dtype=torch.float64) for _ in range(3)]
+        for i in range(n):
+            at = there.clone()
+            at[L - n + i + 1:] = False
+            if not at.any():
+                continue
+            x = q[n + i].double().reshape(H, G, D)
+            w = torch.softmax(x @ kk[:, at].transpose(-1, -2) / math.sqrt(D), -1)
+            want[0][i], want[1][i] = ((w @ v).reshape(H * G, D) for v in (vv[:, at], vv[:, at].abs()))
+            want[2][i] = ((x.abs() @ kk[:, at].abs().transpose(-1, -2)) / math.sqrt(D)).amax(-1).reshape(H * G, 1)
+        ref.check_attention(out[n:], want, dtype, f"without {missing}")
+
+
 def test_pages_past_32_bits(cuda):
     """A cache above 4 GiB: tokens in its last pages."""
     H, D, P, L = 8, 128, 256, 300
