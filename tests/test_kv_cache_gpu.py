@@ -292,6 +292,23 @@ def test_attention_without_a_page(cuda, n, D, dtype):
         ref.check_attention(out[n:], want, dtype, f"without {missing}")
 
 
+def test_append_beside_bad_metadata(cuda):
+    """The other sequence's row is written, each time anew, and nothing else."""
+    H, D, P = 2, 64, 16
+    cache, tiles, table = make(cuda, 890, [40, 40], H, D, P, KV_INT8)
+    bad = table.clone()
+    bad[1, 1] = tiles.shape[0]
+    for i, (t, lengths) in enumerate([(bad, [33, 17]), (table, [34, 49]), (table, [35, -1])]):
+        k = torch.randn((2, H, D), generator=torch.Generator().manual_seed(i))
+        before = cache.tiles.cpu()
+        q4rdna.kv_append(cache, KVBatch(t.to(cuda), i32(lengths, cuda)), k.to(cuda), k.to(cuda))
+        assert q4rdna.take_fault() == 8
+        after = cache.tiles.cpu()
+        changed = (after != before).flatten(1).any(1).nonzero().flatten().tolist()
+        assert changed == [int(table[0, 2])]
+        ref.check_append(before, after, D, KV_INT8, table, lengths[:1], [1], k[:1].double(), k[:1].double())
+
+
 def test_pages_past_32_bits(cuda):
     """A cache above 4 GiB: tokens in its last pages."""
     H, D, P, L = 8, 128, 256, 300
