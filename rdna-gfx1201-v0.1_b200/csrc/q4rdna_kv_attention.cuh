@@ -207,9 +207,9 @@ kv_attention_kernel(const __grid_constant__ AttnArgs A) {
                 mx = max(mx, __float_as_uint(x[t]) & 0x7fffffffu);
             }
             mx = __reduce_max_sync(0xffffffffu, mx);
-            // the largest |q| to [2^13, 2^14); exponents beyond +-100 stay
+            // the largest |q| to [2^13, 2^14)
             int e = 140 - (int)(mx >> 23);
-            e = mx == 0 || mx >= 0x7f800000u ? 0 : max(-100, min(100, e));
+            e = mx == 0 || mx >= 0x7f800000u ? 0 : min(e, kMostExponent);
             const float f = __int_as_float((127 + e) << 23);
 #pragma unroll
             for (int t = 0; t < D / 32; t += 2) {

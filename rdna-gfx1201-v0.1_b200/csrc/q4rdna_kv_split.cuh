@@ -290,6 +290,10 @@ __device__ __forceinline__ uint32_t pair_of(uint32_t w) {
     else return e4m3_pair<LO != 0>(w);
 }
 
+// A row's q is scaled by 2^e, its largest |q| to [2^13, 2^14): e from -114 (2^127) up to here, where 2^e and 2^-e are
+// still normal numbers; below 2^-113 the row lies lower in f16's range (the last bit of a denormal f32 at 2^-23)
+constexpr int kMostExponent = 126;
+
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
                         float f = 1.0f;  // f16 stays as it is
                         if (A.type == Q4RDNA_BF16) {
                             int e = 140 - (int)(mx >> 7);  // the largest |q| to [2^13, 2^14)
-                            e = mx == 0 || mx >= 0x7f80u ? 0 : max(-100, min(100, e));
+                            e = mx == 0 || mx >= 0x7f80u ? 0 : min(e, kMostExponent);
                             f = __int_as_float((127 + e) << 23);
 #pragma unroll
                             for (int i = 0; i < D / 8; ++i) {
@@ -1057,7 +1057,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile32_kernel(const __grid
                                  max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
                     }
                     int e = 140 - (int)(mx >> 23);  // the largest |q| to [2^13, 2^14)
-                    e = mx == 0 || mx >= 0x7f800000u ? 0 : max(-100, min(100, e));
+                    e = mx == 0 || mx >= 0x7f800000u ? 0 : min(e, kMostExponent);
                     const float f = there ? __int_as_float((127 + e) << 23) : 0.0f;
 #pragma unroll 4
                     for (int i = 0; i < D / 8; ++i) {

@@ -144,6 +144,14 @@ def test_attention_scores_far_apart(cuda):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e37, 1e34, 1e-34, 1e-37])
+def test_attention_queries_at_the_ends_of_their_range(cuda, size, dtype):
+    """Huge and tiny queries under a scale that brings their scores back."""
+    for n in (1, 60):
+        attend(cuda, 825, [333], [n], 2, 4, 128, 16, KV_INT8, dtype, q_scale=size, scale=0.1 / size)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("news", [[1, 1, 1, 1], [3, 40, 2, 40]])
 def test_attention_empty_rows(cuda, news, dtype):
     """Padded rows (fewer tokens than rows, none at all): zeros, and the others right."""
