@@ -299,6 +299,11 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// l * 2^d, d <= 0, in two steps: a sum of weights over tiny values' scales is large, and 2^d alone may be no f32 number
+__device__ __forceinline__ float shrunk(float l, float d) {
+    const float h = ex2(0.5f * d);
+    return l * h * h;
+}
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -366,7 +371,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_kernel(const __grid_c
             l = piece(base + lane)[nc * D + nc + j];
         }
         const float f = m == -INFINITY ? 1.0f : ex2(m - M);
-        L = fmaf(f, l, L);
+        L += m == -INFINITY ? l : shrunk(l, m - M);
         const int cnt = min(32, n - base);
         for (int i = w; i < cnt; i += AHEAD * kJoinWarps) {
             float y[AHEAD][EPL];
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv_join_wide_kernel(const __g
             l = piece(base + i)[nc * D + nc + j0 + k];
         }
         const float f = m == -INFINITY ? 1.0f : ex2(m - M);
-        L = fmaf(f, l, L);
+        L += m == -INFINITY ? l : shrunk(l, m - M);
 #pragma unroll
         for (int u0 = 0; u0 < 8; u0 += AHEAD) {
             if (base + u0 >= n) break;

@@ -54,7 +54,7 @@ struct TileSmem {
     uint8_t k[2][STAGE];
     uint8_t v[2][STAGE];
     uint8_t ring[kTileAhead * kTileLoaders * 16];  // pieces of the loading threads on their way
-    float4 scale[4][8];  // per block of a step: key scale, log2 and inverse of the value scale
+    float4 scale[4][8];  // per block of a step: key scale, log2 and inverse of the value scale, largest inverse of the step
     float qscale[2][kTileRows];
     float turn[4][kTileRows], sum[kTileRows * 4], ref[kTileRows * 4];  // f32 rows: O's factor, sum and reference (rings of 4 steps)
     uint64_t bar[28];
@@ -203,6 +203,29 @@ struct RowPlace {
     int tok0, all_lo, all_hi;           // first token of the task; tokens that all rows of the warp see
 };
 
+// A step's weights without the logarithms of the value scales.  The sums by blocks lose those of a block whose values
+// are 2^100 times smaller than the ones that set the reference: they fall below f32's numbers before 1 / sv brings
+// them back (the products may lose them, the sum must not).
+__device__ __forceinline__ float weights_alone(const RowState &r, const float4 *scale, uint32_t s_at, int tok0) {
+    const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
+    float add = 0.0f;
+#pragma unroll 1
+    for (int b = 0; b < 8; ++b) {
+        uint32_t v[16];
+        tmem_load16(s_at + 16 * b, v);
+        tmem_arrived(v);
+        const float4 g = scale[b];
+        const float a = g.x * r.scale;
+        const int tok = tok0 + 16 * b;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            sum += tok + i < r.lo || tok + i > r.hi ? 0.0f : ex2(fmaf(__uint_as_float(v[i]), a, -ref));
+        if (g.y != -INFINITY) add += sum;  // (a page outside the cache)
+    }
+    return add;
+}
+
 // One step of one row: S to P in one pass over S with the reference as it stands: p is
 // right for any reference, as long as it stays in f16's range, and no weight is above
 // the sum of its block.  Where a sum is above 2^15 (or the row has seen nothing yet) the
@@ -242,8 +265,10 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
                 }
             }
             const float f = t > r.R ? ex2(r.R - t) : 1.0f;  // 0 for the first: R = -inf
-            if (t > r.R) r.R = t;
-            r.l *= f;
+            if (t > r.R) {
+                r.l = shrunk(r.l, r.R - t);
+                r.R = t;
+            }
             if (!first) {
                 // the products of the step before have ended (they come before this S), the next ones wait for this P
 #pragma unroll 1
@@ -308,6 +333,9 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
         look = __any_sync(0xffffffffu, most > 32768.0f || r.R == -INFINITY);
         if (!look) break;
     }
+    // The largest weight that may have fallen below 2^-126 in a block, against the sum
+    if (__any_sync(0xffffffffu, r.R != -INFINITY && scale[0].w * 0x1p-92f > r.l + add))
+        add = weights_alone(r, scale, s_at, tok0);
     r.l += add;
     tmem_store32(s_at, *reinterpret_cast<uint32_t(*)[32]>(p));
     tmem_store32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
@@ -438,12 +466,15 @@ __device__ __noinline__ bool load_steps(const AttnArgs &A, const LoadPlace &plac
             __syncwarp();
             if (lane == 0) bar_arrive((z == 0 ? P.k_full : P.v_full) + 8 * stage);
             if (z == 0 && u < 32) {
-                if (u < 8) {
-                    const float sv = head.y <= kTinyScale ? kTinyScale : head.y;  // NaN stays
-                    // a block on a page outside the cache takes no weight, as if it were masked
-                    P.scale[n & 3][u] =
-                        tile0 != 0 ? make_float4(head.x, log2f(sv), 1.0f / sv, 0.0f) : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
-                }
+                const float sv = head.y <= kTinyScale ? kTinyScale : head.y;  // NaN stays
+                const float inv = tile0 != 0 ? 1.0f / sv : 0.0f;
+                float most = inv;  // of lanes 0-7
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                // a block on a page outside the cache takes no weight, as if it were masked
+                if (u < 8)
+                    P.scale[n & 3][u] = tile0 != 0 ? make_float4(head.x, log2f(sv), inv, most)
+                                                   : make_float4(0.0f, -INFINITY, 0.0f, most);
                 __syncwarp();
                 if (lane == 0) bar_arrive(P.sc_full + 8 * (n & 3));
             }
@@ -819,7 +850,7 @@ __device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm
                     if (tok + i < r.lo || tok + i > r.hi) v[i] = 0xff800000u;  // -inf
             }
         };
-        float t = -INFINITY;  // the largest exponent
+        float t = -INFINITY, least = INFINITY;  // the largest exponent; the smallest 1 / sv
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
             tmem_load32(s_at + 32 * c, v);
@@ -832,16 +863,23 @@ __device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm
 #pragma unroll
                 for (int i = 0; i < 16; ++i) m = fmaxf(m, __uint_as_float(v[16 * b + i]));
                 // a block without a visible token has m = -inf, which a scale of 0 would turn into NaN
-                if (m != -INFINITY) t = fmaxf(t, fmaf(m, f.x * r.scale, f.y));
+                if (m != -INFINITY) {
+                    t = fmaxf(t, fmaf(m, f.x * r.scale, f.y));
+                    least = fminf(least, f.z);
+                }
             }
         }
         float f = 1.0f;
         if (t > r.R + 8.0f) {  // also the first: R = -inf
             f = ex2(r.R - t);
+            r.l = shrunk(r.l, r.R - t);
             r.R = t;
-            r.l *= f;
         }
         const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
+        // the largest weight that may fall below 2^-126 in a block, against what the sum holds at least
+        const bool alone = __any_sync(
+            0xffffffffu, t != -INFINITY && scale[0].w * 0x1p-92f > r.l + ex2(t - ref) * least);
+        if (alone) r.l += weights_alone(r, scale, s_at, tok0);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
             uint32_t p[32];
@@ -871,7 +909,7 @@ __device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm
                     p[16 + 8 * b + i / 2] = pack_half(e[0] - h.x, e[1] - h.y);
                 }
                 // a block without a visible token takes nothing from its scale, be it NaN
-                if (sum != 0.0f) r.l = fmaf(sum, g.z, r.l);
+                if (sum != 0.0f && !alone) r.l = fmaf(sum, g.z, r.l);
             }
             tmem_store32(s_at + 32 * c, p);
         }

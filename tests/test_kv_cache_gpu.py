@@ -238,6 +238,36 @@ def test_attention_values_of_zero_scale(cuda):
         ref.check_attention(out, ref.attention(tiles, D, KV_INT8, table, [90], [n], q), torch.float32)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,L", [(3, 200), (70, 200), (70, 3001), (40, 40)])
+def test_attention_value_scales_far_apart(cuda, n, L, D, dtype):
+    """Tiles of tiny, ordinary, huge and no values side by side: each token counts in the softmax by its score alone."""
+    H, G, P = 2, 4, 16
+    cache, tiles, table = make(cuda, 875, [L], H, D, P, KV_INT8)
+    q = torch.randn((n, H * G, D), generator=torch.Generator().manual_seed(2)).to(dtype)
+    batch = KVBatch(table.to(cuda), i32([L], cuda), q_start=i32([0, n], cuda))
+    blocks = -(-L // P)
+    for sizes in ([1e-25, 1e22], [1e22, 1e-25], [0.0, 1e10], [1e30, 0.0, 1.0, 1e-20], [1.0, 1e-28, 0.0]):
+        t = tiles.clone()
+        s, _, v = ref.parts(t, D, KV_INT8)
+        i = torch.arange(blocks)
+        by = torch.tensor(sizes)[i * len(sizes) // blocks if L < 1000 else i % len(sizes)]
+        pages = table[0, :blocks].long()
+        s[pages, :, 0, 1] *= by[:, None]
+        v[pages[by == 0]] = 0  # a tile of scale 0 is stored as zeros
+        cache.tiles.copy_(t)
+        out = q4rdna.kv_attention(cache, batch, q.to(cuda))
+        want, mag, big = ref.attention(t, D, KV_INT8, table, [L], [n], q)
+        # Bounds relative to the row's largest sum p |v|, not each element's.  w sv, the weight times the value's scale, is
+        # held relative to the row's largest one, W (as p >= 2^7 for W itself, in two f16 terms whose last bit is 2^-24):
+        # a term is off by 2^-25 / 2^7 W at most, times a code 2^-25 W, L terms by L 2^-25 W, where an element with
+        # code 0 under W may be 2^-150 W.  The row's largest sum is at least W times its token's largest code, over 2^4: L
+        # 2^-29 = 2^-17.4 relative at 3001, under the 2 A 2^-19 >= 2^-16 of the bound (A >= 4 here; asserted).
+        assert L * 2.0 ** -29 <= 2 * big[-1].min() * 2.0 ** -19
+        ref.check_attention(out, (want, mag.amax(-1, keepdim=True), big), dtype, f"{sizes}")
+
+
 def test_bad_metadata_sets_the_fault(cuda):
     """Pages outside the cache, lengths above the bound and q_start outside the
     rows are refused on the device: bit 3, nothing read or written there."""
