@@ -47,6 +47,9 @@ const at::Tensor &tensor(PyObject *o, const char *name) {
     const at::Tensor &t = THPVariable_Unpack(o);
     if (t.requires_grad() && c10::GradMode::is_enabled())
         throw Refused(std::string("kv cache operators have no gradients: ") + name + " requires one (not under torch.no_grad())");
+    // (torch.no_grad does not turn forward mode off)
+    if (t._fw_grad(0).defined())
+        throw Refused(std::string("kv cache operators have no gradients: ") + name + " carries a tangent");
     return t;
 }
 bool given(PyObject *o) { return o != Py_None; }

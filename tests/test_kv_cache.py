@@ -217,3 +217,22 @@ def test_tiles_are_read_by_ordinary_loads():
         with open(os.path.join(csrc, n)) as f:
             text = f.read()
         assert "ld.global.nc" not in text and "__ldg" not in text, n
+
+
+def test_tangents_are_refused():
+    """Forward mode is not cut silently either, under torch.no_grad() neither."""
+    import torch.autograd.forward_ad as fwd
+
+    cache = q4rdna.KVCache(4, 16, 2, 64, device="cpu")
+    batch = q4rdna.KVBatch(torch.zeros((3, 2), dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+    x = torch.zeros((3, 2, 64))
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: q4rdna.kv_attention(cache, batch, dual), lambda: q4rdna.kv_append(cache, batch, dual, x),
+                     lambda: q4rdna.kv_append(cache, batch, x, dual)):
+            with pytest.raises(ValueError, match="carries a tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="carries a tangent"):
+                call()
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        q4rdna.kv_attention(cache, batch, x)
