@@ -502,6 +502,8 @@ class KVCache:
         desc = KVCacheDesc(None, pages, page_tokens, kv_heads, head_dim, format)
         if format not in (KV_INT8, KV_E4M3):
             raise ValueError(f"unknown cache format {format}")
+        if any(abs(n) >= 1 << 31 for n in (pages, page_tokens, kv_heads, head_dim)):  # 32-bit in the C structures
+            raise ValueError("kv cache: a size is beyond 32 bits")
         nbytes = _lib().q4rdna_kv_cache_bytes(ctypes.byref(desc))
         if nbytes == 0:
             raise ValueError("kv cache: pages and kv_heads positive, page_tokens a power of two in [16, 256], "
@@ -542,8 +544,10 @@ class KVBatch:
             raise ValueError("kv batch: lengths [sequences] and q_start [sequences + 1], contiguous")
         if S > 1 and page_table.stride(0) < page_table.shape[1]:
             raise ValueError("kv batch: the page table's rows overlap")
-        if max_length < 0:
-            raise ValueError("kv batch: max_length is not negative")
+        if not 0 <= max_length <= 1 << 30:
+            raise ValueError("kv batch: max_length is not negative, 2^30 at most")
+        if S > 1 and page_table.stride(0) >= 1 << 31:  # the C structures hold 32-bit numbers
+            raise ValueError("kv batch: the page table's rows lie 2^31 entries apart or more")
         self._keep = (page_table, lengths, q_start)
         self.device = page_table.device
         self.sequences = S

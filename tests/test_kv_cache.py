@@ -236,3 +236,21 @@ def test_tangents_are_refused():
                 call()
     with pytest.raises(ValueError, match="CUDA tensor"):
         q4rdna.kv_attention(cache, batch, x)
+
+
+def test_numbers_past_32_bits_are_refused():
+    """The C structures hold 32-bit numbers: a larger one is not taken modulo 2^32."""
+    i32 = dict(dtype=torch.int32)
+    table, lengths = torch.zeros((3, 2), **i32), torch.zeros(3, **i32)
+    assert q4rdna.KVBatch(table, lengths, max_length=1 << 30)._rec.limit == 1 << 30
+    for n in ((1 << 30) + 1, 1 << 31, (1 << 32) + 5):
+        with pytest.raises(ValueError, match="max_length"):
+            q4rdna.KVBatch(table, lengths, max_length=n)
+    wide = torch.empty_strided((3, 2), ((1 << 32) + 2, 1), dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="page table"):
+        q4rdna.KVBatch(wide, torch.empty(3, dtype=torch.int32, device="meta"))
+    tiles = torch.zeros((4, 2, 1, 16 + 32 * 64), dtype=torch.uint8)
+    for size in ((4 + (1 << 32), 16, 2, 64), (4 - (1 << 32), 16, 2, 64), (4, 16 + (1 << 32), 2, 64), (4, 16, 2 + (1 << 32), 64),
+                 (4, 16, 2, 64 + (1 << 32))):
+        with pytest.raises(ValueError):
+            q4rdna.KVCache(*size, tiles=tiles)
