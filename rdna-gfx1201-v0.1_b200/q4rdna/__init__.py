@@ -514,12 +514,17 @@ class KVCache:
         if tiles.dtype != torch.uint8 or not tiles.is_contiguous() or tiles.numel() != nbytes:
             raise ValueError(f"kv cache tiles: a contiguous uint8 tensor of {nbytes} bytes")
         desc.tiles = tiles.data_ptr()
-        self.tiles = tiles
+        self._tiles = tiles
         self.pages, self.page_tokens, self.kv_heads, self.head_dim = pages, page_tokens, kv_heads, head_dim
         self.format = format
         self.device = tiles.device
         self._rec = _KVCacheRec(desc, _device_index(tiles))
         self._at = ctypes.addressof(self._rec)
+
+    @property
+    def tiles(self):
+        """The cache's bytes: rewritten in place, never replaced (the calls hold their address)."""
+        return self._tiles
 
 
 class KVBatch:

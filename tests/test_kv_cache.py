@@ -254,3 +254,13 @@ def test_numbers_past_32_bits_are_refused():
                  (4, 16, 2, 64 + (1 << 32))):
         with pytest.raises(ValueError):
             q4rdna.KVCache(*size, tiles=tiles)
+
+
+def test_tiles_cannot_be_replaced():
+    """The calls hold the address of the first tiles: with others in their place they would use freed memory."""
+    cache = q4rdna.KVCache(4, 16, 2, 64, device="cpu")
+    at = cache.tiles.data_ptr()
+    with pytest.raises(AttributeError):
+        cache.tiles = cache.tiles.clone()
+    cache.tiles.fill_(1)
+    assert cache.tiles.data_ptr() == at == cache._rec.desc.tiles
