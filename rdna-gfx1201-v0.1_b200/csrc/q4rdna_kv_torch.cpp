@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <algorithm>
 #include <array>
@@ -275,4 +276,12 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_kv_torch", nullptr, -1, metho
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__kv_torch(void) { return PyModule_Create(&module_def); }
+PyMODINIT_FUNC PyInit__kv_torch(void) {
+    PyObject *m = PyModule_Create(&module_def);
+    // the package compares it with the torch that it runs under
+    if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import re
 from ctypes import POINTER, c_char_p, c_int, c_int64, c_size_t, c_uint64, c_void_p
 
 from . import format, synth  # noqa: F401
@@ -474,10 +475,14 @@ def _kv():
     global _kv_module
     if _kv_module is None:
         _lib()
-        import torch  # noqa: F401  (its libraries come first)
+        import torch  # (its libraries come first)
 
         from . import _kv_torch
 
+        built = getattr(_kv_torch, "torch_version", "of unknown version")
+        if re.match(r"[\d.]*\d", torch.__version__).group() != built:
+            raise ImportError(f"q4rdna/_kv_torch.so was built against torch {built}, this is {torch.__version__}: "
+                              "build it again")
         _kv_torch.set_check(check)
         _kv_module = _kv_torch
     return _kv_module

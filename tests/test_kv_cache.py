@@ -264,3 +264,13 @@ def test_tiles_cannot_be_replaced():
         cache.tiles = cache.tiles.clone()
     cache.tiles.fill_(1)
     assert cache.tiles.data_ptr() == at == cache._rec.desc.tiles
+
+
+def test_a_module_of_another_torch_is_refused(monkeypatch):
+    """The call path reads torch's own structures: it runs under the torch that it was built against, or not at all."""
+    monkeypatch.setattr(q4rdna, "_kv_module", None)
+    monkeypatch.setattr(torch, "__version__", "2.0.0+cu118")
+    with pytest.raises(ImportError, match="built against torch"):
+        q4rdna._kv()
+    monkeypatch.undo()
+    assert q4rdna._kv().torch_version == torch.__version__.split("+")[0]
