@@ -44,7 +44,7 @@ q4rdna_status check_batch(const q4rdna_kv_cache *c, const q4rdna_kv_batch *b, in
     if (b->sequences != 0 && (b->page_table == nullptr || b->lengths == nullptr)) return Q4RDNA_ERR_INVALID_ARGUMENT;
     if (b->sequences < 0 || b->table_stride <= 0 || b->max_length < 0 || tokens < 0) return Q4RDNA_ERR_INVALID_ARGUMENT;
     if (b->q_start == nullptr && tokens != b->sequences) return Q4RDNA_ERR_SHAPE;
-    const long long room = std::min<long long>((long long)b->table_stride * c->page_tokens, 1 << 30);
+    const long long room = std::min<long long>((long long)b->table_stride * c->page_tokens, kMaxTokens);
     if (b->max_length > room) return Q4RDNA_ERR_SHAPE;
     // the append's units and the attention's 32-bit row arithmetic
     if (b->sequences > (1 << 28) || tokens > (1 << 28)) return Q4RDNA_ERR_TOO_LARGE;

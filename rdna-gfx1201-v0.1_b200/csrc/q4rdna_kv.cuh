@@ -16,6 +16,7 @@
 namespace q4kv {
 
 constexpr int kBlock = Q4RDNA_KV_BLOCK;
+constexpr int kMaxTokens = 1 << 30;        // of a sequence
 constexpr int kHeader = 16;                // bytes of a tile before its codes
 constexpr float kTinyScale = 0x1p-100f;    // smaller scales are stored as 0
 constexpr unsigned kFaultBatch = 8u;       // q4rdna_take_fault bit 3

@@ -223,10 +223,12 @@ struct Walk {
             const int lane = threadIdx.x & 31;
             const int c = col0 + lane * nc;
             const int mine = c < cols ? work_of(span_of(q, c, nc, A.group, A.window, shift)) : 0;
-            int upto = mine;
+            uint32_t upto = mine;
+            constexpr long long kMost = 32ll * (kMaxTokens / kBlock);
+            static_assert((decltype(upto))kMost == kMost, "the work of 32 tasks");
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += y;
             }
             const unsigned behind = __ballot_sync(0xffffffffu, upto > rest);
