@@ -257,8 +257,17 @@ q4rdna_status plan_attention(const AttnArgs &A, int D, AttnLaunch (&L)[2], int &
     const long long most = A.b.q_start == nullptr ? A.group : (long long)A.b.T * A.group;  // columns of a sequence
     const bool f32 = A.type == Q4RDNA_F32;
     const bool tiles = D <= 128 && most >= kTileFrom;
-    // (one sequence, or a few of many columns on average: no launch for the others, which the tile kernels take too)
-    const bool alone = A.b.S == 1 || A.b.q_start == nullptr || (A.b.S <= 4 && most >= 4LL * kTileFrom * A.b.S);
+    // One sequence, or a few of many columns on average, no length more than twice the average of the new tokens: no
+    // launches for sequences of few columns, which the tile kernels take too.  us for the tile kernel alone and for both
+    // (32 / 8 heads of 128):
+    //                              bf16          f32
+    //   2 x 300, 4 x 300      48, 52   50, 55          72, 77 (4 x 300)
+    //   400 and 1 of 400          47, 59       43, 55
+    //   3000 and 1 of 3000     277, 293     508, 519
+    //   400 and 3 of 8191       122, 73      152, 72     (beyond the bound on the lengths)
+    //   400 and 3 of 65521     728, 177     788, 193
+    const bool alone = A.b.S == 1 || A.b.q_start == nullptr ||
+                       (A.b.S <= 4 && most >= 4LL * kTileFrom * A.b.S && (long long)A.b.max_len * A.b.S <= 2LL * A.b.T);
     if (!tiles || !alone) {
         // One column tile (two CTAs an SM; a sequence of more columns has several tasks) or two, us for 16 sequences of
         // 4001 tokens, 8 kv heads, f32:

@@ -99,6 +99,17 @@ def test_attention_long(cuda):
     attend(cuda, 803, [3001], [70], 2, 4, 128, 32, KV_E4M3, torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lengths,news,launches", [([400, 6000, 5000, 3], [400, 1, 1, 1], 4), ([6000, 400], [1, 400], 4),
+                                                   ([400, 300, 390], [400, 200, 390], 2), ([400, 390], [400, 1], 2)])
+def test_attention_prompt_beside_long_decodes(cuda, lengths, news, launches, dtype):
+    """Single tokens of long sequences go to the kernel for few columns, beside one prompt too; a few sequences of
+    new tokens alone take one kernel."""
+    before = q4rdna.launch_count()
+    attend(cuda, 805, lengths, news, 2, 4, 128, 16, KV_INT8, dtype)
+    assert q4rdna.launch_count() - before == launches
+
+
 def test_attention_many_sequences(cuda):
     g = torch.Generator().manual_seed(5)
     lengths = torch.randint(1, 60, (700,), generator=g).tolist()
