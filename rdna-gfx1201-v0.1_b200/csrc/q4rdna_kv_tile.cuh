@@ -54,7 +54,8 @@ struct TileSmem {
     uint8_t k[2][STAGE];
     uint8_t v[2][STAGE];
     uint8_t ring[kTileAhead * kTileLoaders * 16];  // pieces of the loading threads on their way
-    float4 scale[4][8];  // per block of a step: key scale, log2 and inverse of the value scale, largest inverse of the step
+    float4 scale[4][8];  // per block of a step: key scale, log2 and inverse of the value scale; .w of the first and the
+                         // second: the largest and smallest inverse of the step
     float qscale[2][kTileRows];
     float turn[4][kTileRows], sum[kTileRows * 4], ref[kTileRows * 4];  // f32 rows: O's factor, sum and reference (rings of 4 steps)
     uint64_t bar[28];
@@ -206,8 +207,7 @@ struct RowPlace {
 // A step's weights without the logarithms of the value scales.  The sums by blocks lose those of a block whose values
 // are 2^100 times smaller than the ones that set the reference: they fall below f32's numbers before 1 / sv brings
 // them back (the products may lose them, the sum must not).
-__device__ __forceinline__ float weights_alone(const RowState &r, const float4 *scale, uint32_t s_at, int tok0) {
-    const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
+__device__ __noinline__ float weights_alone(float by, float ref, int lo, int hi, const float4 *scale, uint32_t s_at, int tok0) {
     float add = 0.0f;
 #pragma unroll 1
     for (int b = 0; b < 8; ++b) {
@@ -215,12 +215,12 @@ __device__ __forceinline__ float weights_alone(const RowState &r, const float4 *
         tmem_load16(s_at + 16 * b, v);
         tmem_arrived(v);
         const float4 g = scale[b];
-        const float a = g.x * r.scale;
+        const float a = g.x * by;
         const int tok = tok0 + 16 * b;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            sum += tok + i < r.lo || tok + i > r.hi ? 0.0f : ex2(fmaf(__uint_as_float(v[i]), a, -ref));
+            sum += tok + i < lo || tok + i > hi ? 0.0f : ex2(fmaf(__uint_as_float(v[i]), a, -ref));
         if (g.y != -INFINITY) add += sum;  // (a page outside the cache)
     }
     return add;
@@ -230,15 +230,16 @@ __device__ __forceinline__ float weights_alone(const RowState &r, const float4 *
 // right for any reference, as long as it stays in f16's range, and no weight is above
 // the sum of its block.  Where a sum is above 2^15 (or the row has seen nothing yet) the
 // step's largest exponent is looked for, becomes the reference, and the pass is made
-// again; P goes to tensor memory (over S) only when it is right.
+// again; P goes to tensor memory (over S) only when it is right.  `alone`: once more, with
+// the sum of weights_alone.
 // Tokens that a row of the warp does not see lie outside [all_lo, all_hi]; only the
 // blocks there pay for the mask.
 template <int D>
 __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, uint32_t s_at, uint32_t o_at, int tok0,
                                              int all_lo, int all_hi, bool first) {
     uint32_t p[64];
-    float add;
-    bool look = first;
+    float add, exact = 0.0f;
+    bool look = first, alone = false;
 #pragma unroll 1
     while (true) {
         if (look) {
@@ -280,6 +281,7 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
                     tmem_store32(o_at + c, v);
                 }
             }
+            if (alone) exact = weights_alone(r.scale, (r.R == -INFINITY ? 0.0f : r.R) - 7.0f, r.lo, r.hi, scale, s_at, tok0);
         }
         const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
         uint32_t v[2][16];
@@ -329,13 +331,16 @@ __device__ __forceinline__ void softmax_step(RowState &r, const float4 *scale, u
                 if (one != 0.0f) add = fmaf(one, scale[b - 1].z, add);
             }
         }
-        if (look) break;  // every exponent is now at most the reference
-        look = __any_sync(0xffffffffu, most > 32768.0f || r.R == -INFINITY);
+        if (alone) {
+            add = exact;
+            break;
+        }
+        // The largest weight that may have fallen below 2^-126 in a block, against the sum
+        alone = __any_sync(0xffffffffu, r.R != -INFINITY && scale[0].w * 0x1p-92f > r.l + add);
+        if (look && !alone) break;  // every exponent is now at most the reference
+        look = alone || __any_sync(0xffffffffu, most > 32768.0f || r.R == -INFINITY);
         if (!look) break;
     }
-    // The largest weight that may have fallen below 2^-126 in a block, against the sum
-    if (__any_sync(0xffffffffu, r.R != -INFINITY && scale[0].w * 0x1p-92f > r.l + add))
-        add = weights_alone(r, scale, s_at, tok0);
     r.l += add;
     tmem_store32(s_at, *reinterpret_cast<uint32_t(*)[32]>(p));
     tmem_store32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(p + 32));
@@ -468,13 +473,17 @@ __device__ __noinline__ bool load_steps(const AttnArgs &A, const LoadPlace &plac
             if (z == 0 && u < 32) {
                 const float sv = head.y <= kTinyScale ? kTinyScale : head.y;  // NaN stays
                 const float inv = tile0 != 0 ? 1.0f / sv : 0.0f;
-                float most = inv;  // of lanes 0-7
+                float ends = u == 1 ? -INFINITY : 0.0f;
 #pragma unroll
-                for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                for (int i = 0; i < 8; ++i) {  // lane 0 the largest, lane 1 the smallest, negative
+                    const float x = __shfl_sync(0xffffffffu, inv, i);
+                    if (x > 0.0f) ends = fmaxf(ends, u == 1 ? -x : x);
+                }
+                if (u == 1) ends = -ends;
                 // a block on a page outside the cache takes no weight, as if it were masked
                 if (u < 8)
-                    P.scale[n & 3][u] = tile0 != 0 ? make_float4(head.x, log2f(sv), inv, most)
-                                                   : make_float4(0.0f, -INFINITY, 0.0f, most);
+                    P.scale[n & 3][u] = tile0 != 0 ? make_float4(head.x, log2f(sv), inv, ends)
+                                                   : make_float4(0.0f, -INFINITY, 0.0f, ends);
                 __syncwarp();
                 if (lane == 0) bar_arrive(P.sc_full + 8 * (n & 3));
             }
@@ -850,7 +859,7 @@ __device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm
                     if (tok + i < r.lo || tok + i > r.hi) v[i] = 0xff800000u;  // -inf
             }
         };
-        float t = -INFINITY, least = INFINITY;  // the largest exponent; the smallest 1 / sv
+        float t = -INFINITY;  // the largest exponent
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
             tmem_load32(s_at + 32 * c, v);
@@ -863,10 +872,7 @@ __device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm
 #pragma unroll
                 for (int i = 0; i < 16; ++i) m = fmaxf(m, __uint_as_float(v[16 * b + i]));
                 // a block without a visible token has m = -inf, which a scale of 0 would turn into NaN
-                if (m != -INFINITY) {
-                    t = fmaxf(t, fmaf(m, f.x * r.scale, f.y));
-                    least = fminf(least, f.z);
-                }
+                if (m != -INFINITY) t = fmaxf(t, fmaf(m, f.x * r.scale, f.y));
             }
         }
         float f = 1.0f;
@@ -876,10 +882,11 @@ __device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm
             r.R = t;
         }
         const float ref = (r.R == -INFINITY ? 0.0f : r.R) - 7.0f;
-        // the largest weight that may fall below 2^-126 in a block, against what the sum holds at least
-        const bool alone = __any_sync(
-            0xffffffffu, t != -INFINITY && scale[0].w * 0x1p-92f > r.l + ex2(t - ref) * least);
-        if (alone) r.l += weights_alone(r, scale, s_at, tok0);
+        // the largest weight that may fall below 2^-126 in a block, against what the sum holds at least (2^7 / sv of its
+        // first reference)
+        const bool alone = __any_sync(0xffffffffu, scale[0].w * 0x1p-92f > (r.l > 0.0f ? r.l : 128.0f * scale[1].w));
+        float exact = 0.0f;
+        if (alone) exact = r.l + weights_alone(r.scale, ref, r.lo, r.hi, scale, s_at, tok0);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
             uint32_t p[32];
@@ -909,10 +916,11 @@ __device__ __noinline__ bool softmax32_rows(const RowState &row, TileSmem<D> &sm
                     p[16 + 8 * b + i / 2] = pack_half(e[0] - h.x, e[1] - h.y);
                 }
                 // a block without a visible token takes nothing from its scale, be it NaN
-                if (sum != 0.0f && !alone) r.l = fmaf(sum, g.z, r.l);
+                if (sum != 0.0f) r.l = fmaf(sum, g.z, r.l);
             }
             tmem_store32(s_at + 32 * c, p);
         }
+        if (alone) r.l = exact;
         tmem_wait_store();
         fence_before();
         sm.turn[n & 3][rt] = f;
