@@ -36,11 +36,13 @@
 // The launch is the plans' Launch: one task (single call) or a task table; an
 // item is one CTA, item_begin counts CTA items (RB * S per task).
 
+// x by ordinary loads: this kernel may be resident while the one that writes x still runs, and the read-only path
+// promises data that nobody writes meanwhile (griddepcontrol.wait makes the writes visible to ordinary loads)
 template <int BB>
 __device__ __forceinline__ void cta_fetch_x(const Task &T, int B, int g, int lane, float2 (&xv)[BB]) {
 #pragma unroll
     for (int b = 0; b < BB; ++b)
-        xv[b] = b < B ? __ldg(reinterpret_cast<const float2 *>(T.x + (size_t)b * T.K + (size_t)g * Q4_GROUP) + lane)
+        xv[b] = b < B ? reinterpret_cast<const float2 *>(T.x + (size_t)b * T.K + (size_t)g * Q4_GROUP)[lane]
                       : make_float2(0.0f, 0.0f);
 }
 

@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(128) q4_tc_prep_kernel(const __grid_constant__
     float2 v[BP];
 #pragma unroll
     for (int b = 0; b < BP; ++b) {
-        v[b] = (have && b < B) ? __ldg(reinterpret_cast<const float2 *>(T.x + (size_t)b * T.K + kk))
+        v[b] = (have && b < B) ? *reinterpret_cast<const float2 *>(T.x + (size_t)b * T.K + kk)
                                : make_float2(0.0f, 0.0f);
         float q = fmaf(v[b].x, v[b].x, v[b].y * v[b].y);
         v[b].x *= gv.x;
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) q4_tc_gemv_kernel(const __grid_
                 for (int h = 0; h < HB / 4; ++h) {
                     uint32_t v[16];
                     tmem_ld_x16(taddr + 16 * h, v);
-                    const float4 f4 = __ldg(fg + h);
+                    const float4 f4 = fg[h];  // not __ldg: the prep kernel may still write when this one starts
                     const float fac[4] = {f4.x, f4.y, f4.z, f4.w};
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll

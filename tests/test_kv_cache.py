@@ -274,3 +274,16 @@ def test_a_module_of_another_torch_is_refused(monkeypatch):
         q4rdna._kv()
     monkeypatch.undo()
     assert q4rdna._kv().torch_version == torch.__version__.split("+")[0]
+
+
+def test_activations_are_read_by_ordinary_loads():
+    """The products that overlap the kernel before them (the attention, or their own preparation) read what it wrote."""
+    import os
+    import re
+
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rdna-gfx1201-v0.1_b200", "csrc")
+    for n in ("q4rdna_gemv_cta.cuh", "q4rdna_gemv_tc.cuh"):
+        with open(os.path.join(csrc, n)) as f:
+            text = f.read()
+        assert "griddepcontrol.wait" in text
+        assert not re.search(r"__ldg\([^;]*T\.x", text) and not re.search(r"__ldg\(fg", text), n
