@@ -438,10 +438,12 @@ q4rdna_status q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_bat
  * sees: those up to itself, at most `window` of them.  A row that sees nothing
  * becomes 0; rows outside every sequence keep their values.  f32 rows are
  * computed in at least 22 bits (two f16 terms of q and of the weights, sums in
- * f32), 16-bit rows with weights in f16; results do not depend on the timing.
- * From 96 columns (new tokens x query heads of a kv head) of a sequence on, with
- * head_dim 64 and 128, a weight is held together with its value scale, relative
- * to the row's largest such product.
+ * f32).  16-bit rows have their weights rounded to f16, and from 96 columns (new
+ * tokens x query heads of a kv head) of a sequence on, with head_dim 64 and 128,
+ * their weighted sum is the tensor core's own running sum over the sequence,
+ * which truncates (up to 2^-17 of it).  There a weight is held together with its
+ * value scale, relative to the row's largest such product, in both types.
+ * Results do not depend on the timing.
  * The workspace (q4rdna_kv_attention_workspace_bytes, 16-byte aligned)
  * needs no initialisation and carries nothing from call to call; calls that
  * may overlap on the GPU need one each.  Tokens on a page outside the cache are
