@@ -244,11 +244,21 @@ q4rdna_status size_launch(const AttnArgs &A, int D, AttnLaunch &L) {
 }
 
 // Columns (new tokens x query heads of a kv head) from which on the tile kernels take a
-// sequence.  Measured with 32 query and 8 kv heads of 128, int8, one or four sequences, us
-// for the kernel for few columns and for the tile kernel:
-//   columns             16       32       48       64      128      256     2048
-//   f32              28, 56   40, 58   51, 60   63, 62   81, 59   84, 53  350, 136
-//   bf16             26, 56   35, 58   44, 59   53, 60   66, 51   70, 47  272, 89
+// sequence.  Measured with 32 query and 8 kv heads of 128, int8, us for the kernel for few
+// columns and for the tile kernel (sequences x tokens):
+//   columns               16       64       96      128      256       512
+//   f32   1 x 64      10, 29   13, 31   19, 34   20, 37   34, 37
+//         1 x 512     11, 23   13, 25   18, 27   19, 29   24, 30    33, 30
+//         1 x 4096    17, 32   26, 34   32, 36   37, 38   60, 40   105, 63
+//         1 x 16384   26, 59   57, 64   78, 67   99, 70  184, 92  353, 143
+//         4 x 4096    27, 52   60, 56   86, 59  106, 63  196, 88  370, 145
+//   bf16  1 x 64      10, 24   13, 26   19, 27   19, 29   33, 37
+//         1 x 512     10, 22   12, 24   18, 24   18, 26   23, 31    30, 32
+//         1 x 4096    16, 31   24, 33   29, 34   33, 35   52, 41    91, 42
+//         1 x 16384   24, 53   49, 57   67, 59   84, 60  155, 73   294, 90
+//         4 x 4096    25, 47   53, 50   74, 52   91, 53  166, 68   312, 94
+// The rule knows the columns only: with 500 tokens or fewer the kernel for few columns is
+// faster up to 256 columns, by 17 us at most.
 constexpr int kTileFrom = 96;
 
 // The launches of a call: sequences of few columns, sequences of many, or both
