@@ -23,9 +23,9 @@
 //     dims D/8 g .. of tokens 4 c .. 4 c + 3 (lane = 4 g + c).
 //
 // Measured (8 kv heads of 128, device time with the join): 128 sequences of up to 4093
-// tokens, 64 query heads, e4m3, bf16 140 us, 0.64 of the bytes' time at 6543 GB/s; 32
-// query heads, int8, f32: 16 sequences of up to 8191 47 us and one of 65521 40 us, both
-// 0.51, one of 517 12 us.  About 17 us of a call are fixed: the table of shares, the
+// tokens, 64 query heads, e4m3, bf16 141 us, 0.63 of the bytes' time at 6543 GB/s; 32
+// query heads, int8, f32: 16 sequences of up to 8191 46 us and one of 65521 39 us, 0.52 and
+// 0.53, one of 517 12 us.  About 17 us of a call are fixed: the table of shares, the
 // latency of the first loads, the meeting of the warps, the join.  Sums by int8 products
 // (codes as they are, q in digits) took 164 us where this took 157 (64 of 8191).
 #pragma once

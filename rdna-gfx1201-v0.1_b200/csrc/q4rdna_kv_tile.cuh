@@ -25,8 +25,8 @@
 //     rows only, whose own rounding is 2^-9 or 2^-12; against 64 bits a prompt of 1900 in f16 is off by 2.7e-4
 //     (2.1e-4 with weights in f32, the rest is the output's rounding), bf16 by 1.67e-3 (1.66e-3).
 // Measured (device time with the join): 2048 tokens behind 8191 others, 32 query and 8 kv
-// heads of 128, e4m3, bf16 425 us, 0.44 of the products' time at 1650 TFLOP/s; three
-// prompts of up to 1900, 16 and 4 heads of 64, window 1000, f16 91 us.  Work left out in turn, when the first took 460 us: 354 without
+// heads of 128, e4m3, bf16 426 us, 0.44 of the products' time at 1650 TFLOP/s; three
+// prompts of up to 1900, 16 and 4 heads of 64, window 1000, f16 89 us.  Work left out in turn, when the first took 460 us: 354 without
 // the loading warps' conversion, 308 without the exponentials too, 300 with the products
 // and the waits alone.  So no unit is full: what bounds it are the waits between the
 // roles, the softmax's latency (about 3000 cycles a tile and step) above all.
@@ -834,7 +834,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv_tile_kernel(const __grid_c
 // a task's products would cost 2^-17.  A task is 128 columns, one tile; Q's two terms
 // take the two Q buffers, S two buffers in turn (the next step's S is made under this
 // step's softmax), then the step's O and the task's O.  Warps 4-7 add one to the other.
-// 1024 tokens behind 1024 others, 32 and 8 heads of 128: 143 us (bf16 rows 100 us).
+// 1024 tokens behind 1024 others, 32 and 8 heads of 128: 143 us (bf16 rows 97 us).
 
 constexpr int kTile32Cols = 128;
 
