@@ -428,22 +428,23 @@ size_t q4rdna_kv_cache_bytes(const q4rdna_kv_cache *cache);
  * otherwise.  Where s grew, the older codes become round(code * s_before / s);
  * the new ones are round(x / s), to nearest even.  Rows of a tile behind the
  * last token keep their bytes, rows of q_out outside every sequence their values.
- * A k or v that is not finite makes its tile's
- * scale NaN (so that every row that sees the tile becomes NaN) and its new codes
- * 0 (so that no other row does) until the tile is begun anew.  Two sequences of one call must not write the same tile. */
+ * A k or v that is not finite makes its tile's scale NaN (so that every row that
+ * sees the tile becomes NaN) and its new codes 0 (so that no other row does)
+ * until the tile is begun anew.  Two sequences of one call must not write the
+ * same tile. */
 q4rdna_status q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
                                const q4rdna_kv_append_args *args, q4rdna_stream_t stream);
 
 /* out = softmax(scale * q k^T) v over the cached tokens that the row's token
  * sees: those up to itself, at most `window` of them.  A row that sees nothing
  * becomes 0; rows outside every sequence keep their values.  f32 rows are
- * computed in at least 22 bits (two f16 terms of q and of the weights, sums in
- * f32).  16-bit rows have their weights rounded to f16, and from 96 columns (new
- * tokens x query heads of a kv head) of a sequence on, with head_dim 64 and 128,
- * their weighted sum is the tensor core's own running sum over the sequence,
- * which truncates (up to 2^-17 of it).  There a weight is held together with its
- * value scale, relative to the row's largest such product, in both types.
- * Results do not depend on the timing.
+ * computed in at least 22 bits (two f16 terms of q and of the weights, both
+ * relative to the row's largest, sums in f32).  16-bit rows have their weights
+ * rounded to f16, and from 96 columns (new tokens x query heads of a kv head) of
+ * a sequence on, with head_dim 64 and 128, their weighted sum is the tensor
+ * core's own running sum over the sequence, which truncates (up to 2^-17 of it).
+ * There a weight is held together with its value scale, relative to the row's
+ * largest such product, in both types.  Results do not depend on the timing.
  * The workspace (q4rdna_kv_attention_workspace_bytes, 16-byte aligned)
  * needs no initialisation and carries nothing from call to call; calls that
  * may overlap on the GPU need one each.  Tokens on a page outside the cache are
